@@ -90,6 +90,16 @@ SIGNATURES = {
     "glowb200_set_programmatic_launch": (_int, [_int]),
     "glowb200_quantize_transpose_i8": (_int, [_vp, _vp, _vp, _vp, _int, _f32, _i32, _vp]),
     "glowb200_pairwise_dot_interaction": (_int, [_vp, _i64, _vp, _i64, _i64, _i64, _i64, _vp, _vp, _i64, _f32, _i32, _vp]),
+    "glowb200_microscaled_fp4_scales_bytes": (_sz, [_i64, _i64]),
+    "glowb200_microscaled_fp4_quantize": (_int, [_vp, _int, _i64, _i64, _i64, _vp, _vp, _vp]),
+    "glowb200_microscaled_fp4_dequantize": (_int, [_vp, _vp, _i64, _i64, _vp, _int, _vp]),
+    "glowb200_microscaled_fp4_fc": (_int, [_vp, _int] + [_vp] * 5 + [_i64] * 3 + [_int, _vp, _vp]),
+    "glowb200_dynamic_microscaled_fp4_fc_workspace_bytes": (_sz, [_i64, _i64, _i64]),
+    "glowb200_dynamic_microscaled_fp4_fc": (
+        _int, [_vp, _int, _vp, _int, _i64, _vp, _vp, _vp, _i64, _i64, _i64, _int, _vp, _sz, _vp, _vp]),
+    "glowb200_group_norm_workspace_bytes": (_sz, [_i64] * 4),
+    "glowb200_group_norm": (
+        _int, [_vp, _int, _vp, _f32, _i32, _vp, _int, _vp, _vp] + [_i64] * 4 + [_f32, _int, _vp, _sz, _vp]),
     "glowb200_peer_buffer_create": (_int, [_sz, _vp, _vp]),
     "glowb200_peer_buffer_open": (_int, [_vp, _vp]),
     "glowb200_peer_buffer_close": (_int, [_vp]),

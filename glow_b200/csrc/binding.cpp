@@ -8,6 +8,7 @@
 
 #include <ATen/cuda/EmptyTensor.h>
 #include <ATen/ops/empty_like.h>
+#include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -30,7 +31,10 @@ namespace {
   X(glowb200_channelwise_quantized_conv2d_pair_workspace_bytes) X(glowb200_channelwise_quantized_conv2d_pair_i8_i32) \
   X(glowb200_channelwise_quantized_conv2d_add_i8) X(glowb200_element_add_maxsplat_i8) \
   X(glowb200_element_quantize_i8) X(glowb200_element_dequantize_i8) X(glowb200_max_pool_i8) X(glowb200_avg_pool_i8)    \
-  X(glowb200_quantize_transpose_i8) X(glowb200_pairwise_dot_interaction) X(glowb200_device_manager_run_function_io)
+  X(glowb200_quantize_transpose_i8) X(glowb200_pairwise_dot_interaction) X(glowb200_device_manager_run_function_io)    \
+  X(glowb200_microscaled_fp4_scales_bytes) X(glowb200_microscaled_fp4_quantize) X(glowb200_microscaled_fp4_dequantize)  \
+  X(glowb200_microscaled_fp4_fc) X(glowb200_dynamic_microscaled_fp4_fc_workspace_bytes)                               \
+  X(glowb200_dynamic_microscaled_fp4_fc) X(glowb200_group_norm_workspace_bytes) X(glowb200_group_norm)
 struct Entry {
 #define X(name) decltype(&::name) name = nullptr;
   GLOWB200_ENTRY_POINTS(X)
@@ -46,7 +50,7 @@ struct Raised {};  // a Python exception is set
 using at::Tensor;
 constexpr unsigned bit(at::ScalarType t) { return 1u << (int)t; }
 constexpr unsigned U8 = bit(at::kByte), I8 = bit(at::kChar), I32 = bit(at::kInt), I64 = bit(at::kLong), F16 = bit(at::kHalf),
-                   F32 = bit(at::kFloat);
+                   F32 = bit(at::kFloat), BF16 = bit(at::kBFloat16), FLOATS = F32 | F16 | BF16;
 
 [[noreturn]] void bad_argument(const char *name, PyObject *o, unsigned dtypes) {
   PyObject *r = PyObject_CallFunction(explain, "sOI", name, o, dtypes);
@@ -562,6 +566,156 @@ PyObject *pairwise_dot(PyObject *const *a) {
   return given ? same(a[5]) : give(out);
 }
 
+// ---- microscaled 4-bit layers, group norm ----
+// GLOWB200_FLOAT32 / _FLOAT16 / _BFLOAT16 of a torch type
+int float_type(at::ScalarType t) { return t == at::kFloat ? GLOWB200_FLOAT32 : t == at::kHalf ? GLOWB200_FLOAT16 : GLOWB200_BFLOAT16; }
+// 0, 1, 2: that type; None: the input's
+at::ScalarType result_type(PyObject *o, const Tensor &like) {
+  if (o == Py_None) return like.scalar_type();
+  const int64_t t = integer(o);
+  if (t < 0 || t > 2) {
+    PyErr_SetString(PyExc_TypeError, "out_dtype must be torch.float32, torch.float16 or torch.bfloat16");
+    throw Raised{};
+  }
+  return t == GLOWB200_FLOAT32 ? at::kFloat : t == GLOWB200_FLOAT16 ? at::kHalf : at::kBFloat16;
+}
+[[noreturn]] void bad_value(const char *format, const char *name) {
+  PyErr_Format(PyExc_ValueError, format, name);
+  throw Raised{};
+}
+// `t` is used beside `like`: same device
+const Tensor &beside(const Tensor &t, const char *name, const Tensor &like) {
+  if (t.device() != like.device()) bad_value("%s is on another device than the input", name);
+  return t;
+}
+Tensor given_or_new(PyObject *o, c10::IntArrayRef sizes, at::ScalarType type, const Tensor &like, const char *name) {
+  if (o == Py_None) return empty(sizes, type, like);
+  const Tensor &t = beside(cuda_tensor(o, name, bit(type)), name, like);
+  if (t.sizes() != sizes) bad_value("%s has another shape than the result", name);
+  return t;
+}
+// the current stream of the tensor's device, which is current meanwhile
+struct On {
+  c10::cuda::CUDAGuard guard;
+  explicit On(const Tensor &t) : guard(t.device()) {}
+};
+// a packed matrix: uint8 [rows, 16 * blocks]
+const Tensor &packed(PyObject *o, const char *name) {
+  const Tensor &t = cuda_tensor(o, name, U8);
+  if (t.dim() != 2 || t.size(1) == 0 || t.size(1) % 16 != 0) bad_value("%s must be a uint8 matrix with 16 bytes to every 32 columns", name);
+  return t;
+}
+const Tensor &scale_tiles(PyObject *o, const char *name, const Tensor &data) {
+  const Tensor &t = beside(cuda_tensor(o, name, U8), name, data);
+  if ((size_t)t.numel() != fn.glowb200_microscaled_fp4_scales_bytes(data.size(0), 2 * data.size(1)))
+    bad_value("%s does not hold the scale tiles of its matrix", name);
+  return t;
+}
+const float *floats(PyObject *o, const char *name, int64_t n, const Tensor &like) {
+  if (o == Py_None) return nullptr;
+  const Tensor &t = beside(cuda_tensor(o, name, F32), name, like);
+  if (t.numel() != n) bad_value("%s has another number of elements than the result has columns", name);
+  return (const float *)t.data_ptr();
+}
+int32_t *status_word(PyObject *o, const Tensor &like) {
+  return o == Py_None ? nullptr : (int32_t *)beside(cuda_tensor(o, "status", I32), "status", like).data_ptr();
+}
+// a float CUDA matrix whose columns are neighbours: rows may be apart
+const Tensor &float_rows(PyObject *o, const char *name) {
+  if (!THPVariable_Check(o)) bad_argument(name, o, FLOATS);
+  const Tensor &t = THPVariable_Unpack(o);
+  if (!t.is_cuda() || !(FLOATS >> (int)t.scalar_type() & 1)) bad_argument(name, o, FLOATS);
+  if (t.dim() != 2) bad_value("%s must be a matrix", name);
+  if ((t.size(1) > 1 && t.stride(1) != 1) || (t.size(0) > 1 && t.stride(0) < t.size(1))) bad_value("%s must have its columns side by side and its rows apart", name);
+  return t;
+}
+int64_t row_stride(const Tensor &t) { return t.size(0) > 1 ? t.stride(0) : t.size(1); }
+
+// x, data, scales
+PyObject *mx_quantize(PyObject *const *a) {
+  const Tensor &x = float_rows(a[0], "x");
+  const int64_t rows = x.size(0), cols = x.size(1);
+  const On on(x);
+  const Tensor data = given_or_new(a[1], {rows, 16 * ((cols + 31) / 32)}, at::kByte, x, "out");
+  Tensor scales;
+  const int64_t bytes = (int64_t)fn.glowb200_microscaled_fp4_scales_bytes(rows, cols);
+  if (a[2] == Py_None) scales = empty({(rows + 127) / 128, (cols + 127) / 128, 512}, at::kByte, x);
+  else scales = beside(cuda_tensor(a[2], "scales", U8), "scales", x);
+  if (scales.numel() != bytes) bad_value("%s does not hold the scale tiles of its matrix", "scales");
+  invoke(fn.glowb200_microscaled_fp4_quantize, x.data_ptr(), float_type(x.scalar_type()), rows, cols, row_stride(x),
+         (uint8_t *)data.data_ptr(), (uint8_t *)scales.data_ptr(), stream());
+  return Py_BuildValue("NN", a[1] == Py_None ? give(data) : same(a[1]), a[2] == Py_None ? give(scales) : same(a[2]));
+}
+
+// data, scales, cols, out type, out
+PyObject *mx_dequantize(PyObject *const *a) {
+  const Tensor &data = packed(a[0], "data"), &scales = scale_tiles(a[1], "scales", data);
+  const int64_t rows = data.size(0), cols = integer(a[2]);
+  if (cols <= 0 || 16 * ((cols + 31) / 32) != data.size(1)) bad_value("%s has another number of columns", "data");
+  const On on(data);
+  const at::ScalarType type = a[4] == Py_None ? result_type(a[3], data) : any_tensor(a[4], "out").scalar_type();
+  if (!(FLOATS >> (int)type & 1)) bad_argument("out", a[4], FLOATS);
+  const Tensor out = given_or_new(a[4], {rows, cols}, type, data, "out");
+  invoke(fn.glowb200_microscaled_fp4_dequantize, (const uint8_t *)data.data_ptr(), (const uint8_t *)scales.data_ptr(), rows, cols,
+         out.data_ptr(), float_type(type), stream());
+  return a[4] == Py_None ? give(out) : same(a[4]);
+}
+
+// inp, inp scales, weights, weights scales, bias, flags, out type, out, status
+PyObject *mx_fc(PyObject *const *a) {
+  const Tensor &x = packed(a[0], "inp"), &xs = scale_tiles(a[1], "inp_scales", x), &w = beside(packed(a[2], "weights"), "weights", x),
+               &ws = scale_tiles(a[3], "weights_scales", w);
+  if (x.size(1) != w.size(1)) bad_value("%s has another number of columns than the input", "weights");
+  const int64_t M = x.size(0), K = 2 * x.size(1), N = w.size(0);
+  const On on(x);
+  const at::ScalarType type = a[7] == Py_None ? result_type(a[6], x) : any_tensor(a[7], "out").scalar_type();
+  if (!(FLOATS >> (int)type & 1)) bad_argument("out", a[7], FLOATS);
+  const float *bias = floats(a[4], "bias", N, x);
+  const Tensor out = given_or_new(a[7], {M, N}, type, x, "out");
+  invoke(fn.glowb200_microscaled_fp4_fc, out.data_ptr(), float_type(type), (const uint8_t *)x.data_ptr(), (const uint8_t *)xs.data_ptr(),
+         (const uint8_t *)w.data_ptr(), (const uint8_t *)ws.data_ptr(), bias, M, K, N, (int)integer(a[5]), status_word(a[8], x), stream());
+  return a[7] == Py_None ? give(out) : same(a[7]);
+}
+
+// inp, weights, weights scales, bias, flags, out type, out, workspace, status
+PyObject *mx_dynamic_fc(PyObject *const *a) {
+  const Tensor &x = float_rows(a[0], "inp"), &w = beside(packed(a[1], "weights"), "weights", x), &ws = scale_tiles(a[2], "weights_scales", w);
+  const int64_t M = x.size(0), K = x.size(1), N = w.size(0);
+  if (16 * ((K + 31) / 32) != w.size(1)) bad_value("%s has another number of columns than the input", "weights");
+  const On on(x);
+  const at::ScalarType type = a[6] == Py_None ? result_type(a[5], x) : any_tensor(a[6], "out").scalar_type();
+  if (!(FLOATS >> (int)type & 1)) bad_argument("out", a[6], FLOATS);
+  const float *bias = floats(a[3], "bias", N, x);
+  const Tensor out = given_or_new(a[6], {M, N}, type, x, "out");
+  const Workspace room(a[7], fn.glowb200_dynamic_microscaled_fp4_fc_workspace_bytes(M, K, N), x);
+  beside(room.t, "workspace", x);
+  invoke(fn.glowb200_dynamic_microscaled_fp4_fc, out.data_ptr(), float_type(type), x.data_ptr(), float_type(x.scalar_type()), row_stride(x),
+         (const uint8_t *)w.data_ptr(), (const uint8_t *)ws.data_ptr(), bias, M, K, N, (int)integer(a[4]), room.data(), room.bytes(),
+         status_word(a[8], x), stream());
+  return a[6] == Py_None ? give(out) : same(a[6]);
+}
+
+// x, groups, gamma, beta, eps, activation, quantized?, scale, offset, out type, out, workspace
+PyObject *group_norm(PyObject *const *a) {
+  const Tensor &x = cuda_tensor(a[0], "x", FLOATS);
+  if (x.dim() < 2) bad_value("%s must have images first and channels last", "x");
+  const int64_t images = x.size(0), channels = x.size(x.dim() - 1), groups = integer(a[1]);
+  int64_t pixels = 1;
+  for (int64_t i = 1; i + 1 < x.dim(); i++) pixels *= x.size(i);
+  const On on(x);
+  const bool quant = PyObject_IsTrue(a[6]) == 1;
+  const at::ScalarType type = quant ? at::kChar : a[10] == Py_None ? result_type(a[9], x) : any_tensor(a[10], "out").scalar_type();
+  if (!quant && !(FLOATS >> (int)type & 1)) bad_argument("out", a[10], FLOATS);
+  const float *gamma = floats(a[2], "gamma", channels, x), *beta = floats(a[3], "beta", channels, x);
+  const Tensor out = given_or_new(a[10], x.sizes(), type, x, "out");
+  const Workspace room(a[11], fn.glowb200_group_norm_workspace_bytes(images, pixels, channels, groups), x);
+  beside(room.t, "workspace", x);
+  invoke(fn.glowb200_group_norm, quant ? nullptr : out.data_ptr(), quant ? 0 : float_type(type), quant ? (int8_t *)out.data_ptr() : nullptr,
+         real(a[7]), (int32_t)integer(a[8]), x.data_ptr(), float_type(x.scalar_type()), gamma, beta, images, pixels, channels, groups,
+         real(a[4]), (int)integer(a[5]), room.data(), room.bytes(), stream());
+  return a[10] == Py_None ? give(out) : same(a[10]);
+}
+
 // ---- device manager ----
 // handle, network name, {placeholder name: array}, names of the outputs (None: every array goes in and comes back)
 PyObject *run_function(PyObject *const *a) {
@@ -664,6 +818,11 @@ PyMethodDef methods[] = {
     FAST("avg_pool", pool<true>, 9),
     FAST("quantize_transpose", quantize_transpose, 5),
     FAST("pairwise_dot", pairwise_dot, 6),
+    FAST("mx_quantize", mx_quantize, 3),
+    FAST("mx_dequantize", mx_dequantize, 5),
+    FAST("mx_fc", mx_fc, 9),
+    FAST("mx_dynamic_fc", mx_dynamic_fc, 9),
+    FAST("group_norm", group_norm, 12),
     FAST("run_function", run_function, 4),
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_binding", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

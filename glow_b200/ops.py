@@ -23,8 +23,9 @@ STATUS_UNSUPPORTED_TABLE = 32
 
 def _explain(name, obj, dtypes):
     """Raises what is wrong with an argument the native binding turned down."""
-    names = (torch.uint8, torch.int8, torch.int16, torch.int32, torch.int64, torch.float16, torch.float32)
-    _cuda(obj, name, tuple(t for i, t in enumerate(names) if dtypes >> i & 1) or None)
+    names = {0: torch.uint8, 1: torch.int8, 2: torch.int16, 3: torch.int32, 4: torch.int64, 5: torch.float16, 6: torch.float32,
+             15: torch.bfloat16}
+    _cuda(obj, name, tuple(t for i, t in names.items() if dtypes >> i & 1) or None)
     raise TypeError("%s is not a suitable tensor" % name)
 
 
@@ -619,6 +620,60 @@ def pairwise_dot_interaction(dense, pooled, *, quant=None, out=None):
     (n = T + 1), or int8 when quant=(scale, offset) (the following Quantize node fused)."""
     q = quant or (1.0, 0)
     return _native().pairwise_dot(dense, pooled, bool(quant), q[0], q[1], out)
+
+
+# ------------------------------------------------------------------------------------------
+# Microscaled 4-bit layers and group norm
+# ------------------------------------------------------------------------------------------
+_FLOAT_TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+NORM_ACT_NONE, NORM_ACT_RELU, NORM_ACT_SWISH = 0, 1, 2
+
+
+def _float_type(dtype):
+    if dtype is not None and dtype not in _FLOAT_TYPES:
+        raise TypeError("out_dtype must be torch.float32, torch.float16 or torch.bfloat16")
+    return None if dtype is None else _FLOAT_TYPES[dtype]
+
+
+def microscaled_fp4_scales_bytes(rows, cols):
+    """Bytes of the scale tiles of a microscaled matrix [rows, cols]."""
+    return int(_lib.lib().glowb200_microscaled_fp4_scales_bytes(int(rows), int(cols)))
+
+
+def microscaled_fp4_quantize(x, *, out=None, scales=None):
+    """A float32, float16 or bfloat16 matrix [rows, cols] (rows may be apart) in the microscaled 4-bit format: returns
+    (data uint8 [rows, 16 * ceil(cols / 32)], scales uint8 [ceil(rows / 128), ceil(cols / 128), 512]).  Every 32 neighbours
+    of a row share a power of two; a NaN or an infinity makes its 32 neighbours NaN."""
+    return _native().mx_quantize(x, out, scales)
+
+
+def microscaled_fp4_dequantize(data, scales, cols, *, out_dtype=torch.float32, out=None):
+    """The numbers [rows, cols] that a microscaled matrix stands for; float32 and bfloat16 hold them exactly."""
+    return _native().mx_dequantize(data, scales, cols, _float_type(out_dtype), out)
+
+
+def microscaled_fp4_fc(inp, inp_scales, weights, weights_scales, bias=None, *, flags=0, out_dtype=torch.float16, out=None,
+                       status=None):
+    """Fully connected layer over microscaled operands: inp [M, K] and weights [N, K] as microscaled_fp4_quantize gives
+    them, bias fp32 [N]; result [M, N] of out_dtype (or out's).  flags: FC_FUSE_RELU."""
+    return _native().mx_fc(inp, inp_scales, weights, weights_scales, bias, flags, _float_type(out_dtype), out, status)
+
+
+def dynamic_microscaled_fp4_fc(inp, weights, weights_scales, bias=None, *, flags=0, out_dtype=None, out=None, workspace=None,
+                               status=None):
+    """microscaled_fp4_fc on a float input [M, K] (float32, float16 or bfloat16, rows may be apart) that the layer quantizes
+    itself; result [M, N] of out_dtype, by default the input's."""
+    return _native().mx_dynamic_fc(inp, weights, weights_scales, bias, flags, _float_type(out_dtype), out, workspace, status)
+
+
+def group_norm(x, groups, gamma=None, beta=None, eps=1e-5, *, activation=NORM_ACT_NONE, quant=None, out_dtype=None, out=None,
+               workspace=None):
+    """Group norm of channels-last activations [images, ..., channels] (float32, float16 or bfloat16) with an activation
+    behind it (NORM_ACT_*); gamma, beta fp32 [channels].  Result of out_dtype, by default the input's, or int8 when
+    quant=(scale, offset) (the following Quantize node fused)."""
+    q = quant or (1.0, 0)
+    return _native().group_norm(x, groups, gamma, beta, eps, activation, quant is not None, q[0], q[1], _float_type(out_dtype), out,
+                                workspace)
 
 
 def device_tensor(ptr, shape, dtype, device="cuda"):

@@ -640,6 +640,67 @@ int glowb200_quantize_transpose_i8(int8_t *dest, const float *src, const int64_t
                                    glowb200_stream_t stream);
 
 /* ---------------------------------------------------------------------------------------
+ * Microscaled 4-bit layers and channels-last group norm.  No reference counterpart: Glow's quantized
+ * dense layers are int8, and it has no GroupNorm node.
+ * ------------------------------------------------------------------------------------- */
+
+/* Element types of float operands of this section. */
+#define GLOWB200_FLOAT32 0
+#define GLOWB200_FLOAT16 1
+#define GLOWB200_BFLOAT16 2
+
+/* The microscaled 4-bit format (the OCP microscaling format MXFP4) of a matrix [rows, cols]: every block of 32 neighbours of
+ * a row shares the scale 2^e, e = floor(log2(max |x|)) - 2, at least -127; an element is the E2M1 number (0, 0.5, 1,
+ * 1.5, 2, 3, 4, 6 and their negatives) nearest to x / 2^e, ties to the even code, beyond 6 it is 6.
+ *   data    [rows, 16 * ceil(cols / 32)] bytes: two elements to a byte, the even column in the low half; code = sign << 3 |
+ *           exponent << 1 | mantissa; zeros behind the last column.
+ *   scales  glowb200_microscaled_fp4_scales_bytes(rows, cols) bytes, e + 127 of every block, in tiles of 128 rows by 4
+ *           blocks, 512 bytes each: row r, block b is byte (r % 32) * 16 + (r / 32 % 4) * 4 + b % 4 of tile
+ *           (r / 128) * ceil(blocks / 4) + b / 4.  Bytes of rows and blocks that are not there are 0.
+ * Both start on 16-byte boundaries.  A block that holds a NaN or an infinity has the scale byte 255 and stands for 32
+ * NaNs.  This tile order is the one in which the tensor cores take the scales. */
+size_t glowb200_microscaled_fp4_scales_bytes(int64_t rows, int64_t cols);
+/* in [rows, cols] of in_type, rows `row_stride` elements apart (at least cols). */
+int glowb200_microscaled_fp4_quantize(const void *in, int in_type, int64_t rows, int64_t cols, int64_t row_stride,
+                                      uint8_t *data, uint8_t *scales, glowb200_stream_t stream);
+/* out [rows, cols] of out_type, dense: the numbers the format stands for, rounded to out_type once (fp32 and bf16 hold
+ * them exactly). */
+int glowb200_microscaled_fp4_dequantize(const uint8_t *data, const uint8_t *scales, int64_t rows, int64_t cols, void *out,
+                                        int out_type, glowb200_stream_t stream);
+
+/* Fully connected layer over microscaled operands: out[i,j] = sum_k in[i,k] * weights[j,k] + bias[j], fp32 sums, rounded
+ * to out_type once.  in [M,K] and weights [N,K] in the format above; bias fp32 [N] or NULL; out [M,N] dense.
+ * flags: GLOWB200_FC_FUSE_RELU (NaN stays NaN).  The bytes behind column K are read: they are zeros, as the quantizer
+ * leaves them. */
+int glowb200_microscaled_fp4_fc(void *out, int out_type, const uint8_t *in, const uint8_t *in_scales, const uint8_t *weights,
+                                const uint8_t *weights_scales, const float *bias, int64_t M, int64_t K, int64_t N, int flags,
+                                int32_t *status, glowb200_stream_t stream);
+/* The same with a float input [M,K] of in_type (rows `row_stride` elements apart), quantized by the layer: the result of
+ * glowb200_microscaled_fp4_quantize followed by glowb200_microscaled_fp4_fc, bit for bit.  The workspace (256-byte
+ * aligned) must hold glowb200_dynamic_microscaled_fp4_fc_workspace_bytes(M, K, N). */
+size_t glowb200_dynamic_microscaled_fp4_fc_workspace_bytes(int64_t M, int64_t K, int64_t N);
+int glowb200_dynamic_microscaled_fp4_fc(void *out, int out_type, const void *in, int in_type, int64_t row_stride,
+                                        const uint8_t *weights, const uint8_t *weights_scales, const float *bias, int64_t M,
+                                        int64_t K, int64_t N, int flags, void *workspace, size_t workspace_bytes,
+                                        int32_t *status, glowb200_stream_t stream);
+
+/* Group norm of channels-last activations with the activation behind it: in [images, pixels, channels] of in_type, dense;
+ * the channels of an image are normalised in `groups` equal runs of neighbours, each with the mean and the (biased)
+ * variance of its channels over all pixels, fp32:
+ *   y = act((x - mean) / sqrt(variance + eps) * gamma[c] + beta[c])
+ * gamma, beta: fp32 [channels] or NULL (1 and 0).  The result, dense like `in`, is rounded once to out_type, or to int8
+ * as glowb200_element_quantize_i8 does it with quant_scale / quant_offset: exactly one of out and out_i8 is given.
+ * act: GLOWB200_NORM_ACT_*.  The workspace (256-byte aligned) must hold glowb200_group_norm_workspace_bytes(...). */
+#define GLOWB200_NORM_ACT_NONE 0
+#define GLOWB200_NORM_ACT_RELU 1
+#define GLOWB200_NORM_ACT_SWISH 2 /* y / (1 + exp(-y)) */
+size_t glowb200_group_norm_workspace_bytes(int64_t images, int64_t pixels, int64_t channels, int64_t groups);
+int glowb200_group_norm(void *out, int out_type, int8_t *out_i8, float quant_scale, int32_t quant_offset, const void *in,
+                        int in_type, const float *gamma, const float *beta, int64_t images, int64_t pixels, int64_t channels,
+                        int64_t groups, float eps, int act, void *workspace, size_t workspace_bytes,
+                        glowb200_stream_t stream);
+
+/* ---------------------------------------------------------------------------------------
  * Recommendation-model pieces
  * ------------------------------------------------------------------------------------- */
 

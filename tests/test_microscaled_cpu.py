@@ -1,0 +1,83 @@
+"""The microscaled 4-bit entry points and group norm turn down on the host what they cannot take; no GPU is needed."""
+import ctypes as C
+
+import numpy as np
+import pytest
+
+import microscaled_reference as ref
+
+
+@pytest.fixture(scope="module")
+def l():
+    from glow_b200 import _lib, build
+    build.build()
+    return _lib.lib()
+
+
+FAKE, ODD = C.c_void_p(4096), C.c_void_p(4096 + 8)
+
+
+def test_sizes(l):
+    assert l.glowb200_microscaled_fp4_scales_bytes(1, 1) == 512
+    assert l.glowb200_microscaled_fp4_scales_bytes(129, 129) == 4 * 512
+    assert l.glowb200_microscaled_fp4_scales_bytes(0, 64) == 0 and l.glowb200_microscaled_fp4_scales_bytes(-1, 64) == 0
+    assert l.glowb200_dynamic_microscaled_fp4_fc_workspace_bytes(5, 100, 7) >= 5 * 64 + 512
+    assert l.glowb200_dynamic_microscaled_fp4_fc_workspace_bytes(-5, 100, 7) == 0
+    assert l.glowb200_group_norm_workspace_bytes(0, 9, 8, 2) == 0
+
+
+@pytest.mark.parametrize("args", [(FAKE, 3, 4, 64, 64, FAKE, FAKE), (FAKE, 0, -1, 64, 64, FAKE, FAKE), (FAKE, 0, 4, 0, 64, FAKE, FAKE),
+                                  (FAKE, 0, 4, 64, 63, FAKE, FAKE), (None, 0, 4, 64, 64, FAKE, FAKE), (FAKE, 0, 4, 64, 64, ODD, FAKE),
+                                  (FAKE, 0, 4, 64, 64, FAKE, ODD), (C.c_void_p(4098), 0, 4, 64, 64, FAKE, FAKE)])
+def test_quantize_refuses(l, args):
+    assert l.glowb200_microscaled_fp4_quantize(*args, None) == 1
+    assert l.glowb200_last_error()
+
+
+def test_nothing_to_do_needs_no_gpu(l):
+    assert l.glowb200_microscaled_fp4_quantize(None, 0, 0, 64, 64, None, None, None) == 0
+    assert l.glowb200_microscaled_fp4_dequantize(None, None, 0, 64, None, 0, None) == 0
+    assert l.glowb200_microscaled_fp4_fc(None, 0, None, None, None, None, None, 0, 64, 8, 0, None, None) == 0
+    assert l.glowb200_dynamic_microscaled_fp4_fc(None, 0, None, 0, 64, None, None, None, 8, 64, 0, 0, None, 0, None, None) == 0
+    assert l.glowb200_group_norm(None, 0, None, 1.0, 0, None, 0, None, None, 0, 9, 8, 2, 1e-5, 0, None, 0, None) == 0
+
+
+@pytest.mark.parametrize("change", [dict(out_type=3), dict(K=0), dict(M=-1), dict(N=1 << 31), dict(flags=2), dict(out=None), dict(a=None),
+                                    dict(sa=None), dict(b=None), dict(sb=None), dict(a=ODD), dict(sa=ODD), dict(b=ODD), dict(sb=ODD),
+                                    dict(out=C.c_void_p(4098))])
+def test_fc_refuses(l, change):
+    v = dict(out=FAKE, out_type=0, a=FAKE, sa=FAKE, b=FAKE, sb=FAKE, bias=None, M=4, K=64, N=8, flags=0)
+    v.update(change)
+    assert l.glowb200_microscaled_fp4_fc(*v.values(), None, None) == 1
+    assert l.glowb200_last_error()
+
+
+def test_dynamic_fc_refuses(l):
+    def call(in_type=0, stride=64, ws=FAKE, size=1 << 20, inp=FAKE):
+        return l.glowb200_dynamic_microscaled_fp4_fc(FAKE, 0, inp, in_type, stride, FAKE, FAKE, None, 4, 64, 8, 0, ws, size, None, None)
+    assert call(in_type=5) == 1 and call(stride=63) == 1 and call(inp=C.c_void_p(4097)) == 1 and call(inp=None) == 1
+    assert call(ws=None) == 3 and call(size=10) == 3 and b"needed" in l.glowb200_last_error()
+    assert call(ws=C.c_void_p(4096 + 16)) == 1
+
+
+@pytest.mark.parametrize("change,code", [(dict(groups=3), 1), (dict(groups=0), 1), (dict(channels=0), 1), (dict(images=-1), 1), (dict(act=3), 1),
+                                         (dict(eps=-1.0), 1), (dict(eps=float("nan")), 1), (dict(in_type=4), 1), (dict(out_type=4), 1),
+                                         (dict(out_i8=FAKE), 1), (dict(out=None), 1), (dict(inp=None), 1), (dict(inp=C.c_void_p(4097)), 1),
+                                         (dict(ws=None), 3), (dict(size=7), 3), (dict(ws=C.c_void_p(4096 + 64)), 1)])
+def test_group_norm_refuses(l, change, code):
+    v = dict(out=FAKE, out_type=0, out_i8=None, scale=1.0, offset=0, inp=FAKE, in_type=1, gamma=None, beta=None, images=2, pixels=9, channels=8,
+             groups=2, eps=1e-5, act=0, ws=FAKE, size=1 << 20)
+    v.update(change)
+    assert l.glowb200_group_norm(*v.values(), None) == code
+    assert l.glowb200_last_error()
+
+
+def test_the_reference_itself():
+    """The tests' own quantizer on numbers worked out by hand."""
+    x = np.zeros((1, 64), np.float32)
+    x[0, :10] = [7.9, 5, 2.5, -3.5, 0.25, 0.75, -0.2, 1.25, 1.75, 6.1]  # e = 0: 7.9 and 6.1 saturate, ties go to even codes
+    x[0, 32:34] = [8, -3]                                               # e = 1: 4, -1.5
+    codes, sc = ref.quantize(x)
+    assert list(ref.values(codes, sc)[0, :10]) == [6, 4, 2, -4, 0, 1, 0, 1, 2, 6]
+    assert list(ref.values(codes, sc)[0, 32:34]) == [8, -3] and list(sc[0]) == [127, 128]
+    assert codes[0, 6] == 8  # -0.2 becomes -0
