@@ -14,7 +14,8 @@ namespace {
 constexpr int kBlockM = 128;
 constexpr int kBlockK = 128;  // bytes of a row per pipeline stage: 256 elements, one 128-byte swizzle atom
 constexpr int kUmmaK = 32;    // bytes of a row per MMA: 64 elements, two scales
-constexpr int kThreads = 192;
+constexpr int kEpilogueWarps = 8;  // two to a lane quarter of tensor memory
+constexpr int kThreads = 64 + 32 * kEpilogueWarps;
 
 __device__ __forceinline__ void umma_mxf4(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t a_scales,
                                           uint32_t b_scales, uint32_t accumulate) {
@@ -43,48 +44,107 @@ struct FcParams {
   const float *bias;
   int32_t *status;
   int M, N, k_steps;  // k_steps: MMAs to a row, 64 elements each
-  int relu;
+  int relu, store_by_tma;
 };
 
-template <int BLOCK_N, int STAGES>
-struct Smem {
-  static constexpr int kRowTiles = (BLOCK_N + 127) / 128;
+// Tensor memory (512 columns): two accumulators, then the scales of the k-blocks in flight.  Two accumulators of 256
+// columns would leave no room for the scales, so they share kShared columns there: the epilogue empties those first, and
+// the next tile's MMAs start as soon as it has.
+template <int BLOCK_N, int STAGES, typename Out>
+struct Tile {
+  static constexpr int kRowTiles = (BLOCK_N + 127) / 128;  // of the right operand's scales
   static constexpr int kABytes = kBlockM * kBlockK, kBBytes = BLOCK_N * kBlockK;
   static constexpr int kSaBytes = 1024, kSbBytes = 1024 * kRowTiles;
   static constexpr int kStageBytes = kABytes + kBBytes + kSaBytes + kSbBytes;
-  static constexpr int kTotal = STAGES * kStageBytes + 256 + 1024;
+  static constexpr int kChunk = 128 / (int)sizeof(Out);  // columns that a warp drains at a time: rows of 128 bytes
+  static constexpr int kStaging = kEpilogueWarps * 32 * 128;
+  static constexpr int kTotal = STAGES * kStageBytes + kStaging + 2 * BLOCK_N * 4 + 256 + 1024;
   static_assert(kTotal <= 232448, "more shared memory than a CTA can have");
+  static constexpr int kShared = BLOCK_N == 256 ? 64 : 0;
+  static constexpr uint32_t kScaleCols = 8 + 8 * kRowTiles;  // of one k-block
+  static constexpr uint32_t kScalesAt = 2 * BLOCK_N - kShared;
+  static constexpr int kSlots = BLOCK_N == 256 ? 2 : 4;
+  static_assert(kScalesAt + kSlots * kScaleCols <= 512 && kSlots <= STAGES && kShared % kChunk == 0, "tensor memory");
 };
 
+__device__ __forceinline__ uint32_t pack2(float lo, float hi, __half) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+__device__ __forceinline__ uint32_t pack2(float lo, float hi, __nv_bfloat16) {
+  uint32_t r;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+__device__ __forceinline__ void tma_store_2d(const CUtensorMap *map, const void *src, int c0, int c1) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];"
+               ::"l"(map), "r"(c0), "r"(c1), "r"(smem_u32(src))
+               : "memory");
+}
+
+// One lane of a warp that runs together.  The loops that issue TMA loads and MMAs are walked by whole warps and only the
+// instructions are this lane's: their operands then stay in uniform registers.  In a loop of one lane of a divergent
+// warp every tcgen05 instruction took 60 to 95 clocks to issue, 1100 to 1270 a k-block, whatever the MMAs' size.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t one;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
+  return one != 0;
+}
+
+// mbar_wait by a whole warp, whose lanes agree on the outcome.
+__device__ __forceinline__ bool warp_wait(uint64_t *bar, uint32_t parity, volatile int *abort_flag) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag));
+}
+
+// Position in a ring of N places, and how often (even or odd) it has come round.
+template <int N>
+struct Ring {
+  int at = 0;
+  uint32_t round = 0;
+  __device__ __forceinline__ void next() {
+    if (++at == N) {
+      at = 0;
+      round ^= 1;
+    }
+  }
+};
+
+// Persistent: blocks walk the 128 x BLOCK_N tiles, row tile fastest (blocks that run together share weights).  Warp 0
+// loads, warp 1 issues the copies of the scales and the MMAs, warps 2 to 9 drain.
 template <int BLOCK_N, int STAGES, typename Out>
 __global__ void __launch_bounds__(kThreads, 1)
 fp4_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
-                const __grid_constant__ CUtensorMap map_sa, const __grid_constant__ CUtensorMap map_sb, const FcParams p) {
-  using S = Smem<BLOCK_N, STAGES>;
+                const __grid_constant__ CUtensorMap map_sa, const __grid_constant__ CUtensorMap map_sb,
+                const __grid_constant__ CUtensorMap map_out, const FcParams p) {
+  using S = Tile<BLOCK_N, STAGES, Out>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-  uint8_t *scales = smem + STAGES * (S::kABytes + S::kBBytes);
-  uint64_t *full = reinterpret_cast<uint64_t *>(scales + STAGES * (S::kSaBytes + S::kSbBytes));
+  uint8_t *staging = smem + STAGES * (S::kABytes + S::kBBytes);
+  uint8_t *scales = staging + S::kStaging;
+  float *bias = reinterpret_cast<float *>(scales + STAGES * (S::kSaBytes + S::kSbBytes));  // [2][BLOCK_N]
+  uint64_t *full = reinterpret_cast<uint64_t *>(bias + 2 * BLOCK_N);
   uint64_t *empty = full + STAGES;
-  uint64_t *acc_full = empty + STAGES;
-  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(acc_full + 1);
+  uint64_t *acc_full = empty + STAGES;  // [2]
+  uint64_t *acc_empty = acc_full + 2;   // [2]
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(acc_empty + 2);
   volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
-  constexpr uint32_t kScaleCols = 8 + 8 * S::kRowTiles;  // of one stage
-  constexpr uint32_t kTmemCols = 512;
-  static_assert(BLOCK_N + STAGES * kScaleCols <= kTmemCols, "tensor memory");
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; s++) {
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
     }
-    mbar_init(acc_full, 1);
+    for (int b = 0; b < 2; b++) {
+      mbar_init(&acc_full[b], 1);
+      mbar_init(&acc_empty[b], kEpilogueWarps);
+    }
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 1) {
-    tmem_alloc(tmem_slot, kTmemCols);
+    tmem_alloc(tmem_slot, 512);
     tmem_relinquish();
   }
   tc_fence_before();
@@ -92,84 +152,171 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
   tc_fence_after();
   pdl_wait();
   pdl_launch_dependents();
-  const uint32_t tmem_base = *tmem_slot;
-  const int m0 = blockIdx.x * kBlockM, n0 = blockIdx.y * BLOCK_N;
+  const uint32_t tmem_base = __shfl_sync(0xffffffffu, *tmem_slot, 0);
+  const int m_tiles = (p.M + kBlockM - 1) / kBlockM, n_tiles = (p.N + BLOCK_N - 1) / BLOCK_N;
+  const int64_t tiles = (int64_t)m_tiles * n_tiles;
   const int k_blocks = (p.k_steps + 3) >> 2;
 
   if (warp == 0) {
-    if (lane == 0) {
-      for (int kb = 0; kb < k_blocks; kb++) {
-        const int s = kb % STAGES;
-        if (kb >= STAGES && !mbar_wait(&empty[s], ((kb / STAGES) - 1) & 1, abort_flag)) break;
+    Ring<STAGES> ring;
+    bool live = true;
+    for (int64_t t = blockIdx.x; t < tiles && live; t += gridDim.x) {
+      const int n_tile = (int)(t / m_tiles), m0 = (int)(t - (int64_t)n_tile * m_tiles) * kBlockM, n0 = n_tile * BLOCK_N;
+      for (int kb = 0; kb < k_blocks; kb++, ring.next()) {
+        const int s = ring.at;
+        if (!warp_wait(&empty[s], ring.round ^ 1, abort_flag)) { live = false; break; }  // (passes at once the first time round)
         uint8_t *a = smem + s * (S::kABytes + S::kBBytes), *sa = scales + s * (S::kSaBytes + S::kSbBytes);
-        mbar_expect_tx(&full[s], S::kStageBytes);
-        tma_load_2d(a, &map_a, kb * kBlockK, m0, &full[s]);
-        tma_load_2d(a + S::kABytes, &map_b, kb * kBlockK, n0, &full[s]);
-        tma_load_2d(sa, &map_sa, kb * 256, m0 >> 7, &full[s]);
-        tma_load_2d(sa + S::kSaBytes, &map_sb, kb * 256, n0 >> 7, &full[s]);
+        if (elect_one()) {
+          mbar_expect_tx(&full[s], S::kStageBytes);
+          tma_load_2d(sa, &map_sa, kb * 256, m0 >> 7, &full[s]);
+          tma_load_2d(sa + S::kSaBytes, &map_sb, kb * 256, n0 >> 7, &full[s]);
+          tma_load_2d(a, &map_a, kb * kBlockK, m0, &full[s]);
+          tma_load_2d(a + S::kABytes, &map_b, kb * kBlockK, n0, &full[s]);
+        }
+        __syncwarp();
       }
     }
   } else if (warp == 1) {
-    if (lane == 0) {
-      bool live = true;
-      for (int kb = 0; kb < k_blocks; kb++) {
-        const int s = kb % STAGES;
-        if (!mbar_wait(&full[s], (kb / STAGES) & 1, abort_flag)) { live = false; break; }
+    Ring<STAGES> ring, done;  // done: the k-block whose MMAs have to be complete before its scales' columns are taken again
+    Ring<S::kSlots> slot;
+    int started = 0;
+    int lt = 0;
+    bool live = true;
+    for (int64_t t = blockIdx.x; t < tiles && live; t += gridDim.x, lt++) {
+      const int buf = lt & 1;
+      const int half_tile = BLOCK_N % 128 ? (int)(t / m_tiles) * BLOCK_N & 127 : 0;  // rows of the first scale tile in front of this tile's
+      // The columns this tile's sums go to: of the shared ones the tile before has to be gone, else the one before that.
+      if (S::kShared ? lt >= 1 && !warp_wait(&acc_empty[buf ^ 1], ((lt - 1) >> 1) & 1, abort_flag)
+                     : lt >= 2 && !warp_wait(&acc_empty[buf], ((lt >> 1) - 1) & 1, abort_flag)) break;
+      tc_fence_after();
+      const uint32_t d_tmem = tmem_base + (uint32_t)(buf * (BLOCK_N - S::kShared));
+      for (int kb = 0; kb < k_blocks; kb++, ring.next(), slot.next()) {
+        const int s = ring.at;
+        if (!warp_wait(&full[s], ring.round, abort_flag)) { live = false; break; }
+        if (started < S::kSlots) {
+          started++;
+        } else {
+          if (!warp_wait(&empty[done.at], done.round, abort_flag)) { live = false; break; }
+          done.next();
+        }
         tc_fence_after();
         const uint32_t a_addr = smem_u32(smem + s * (S::kABytes + S::kBBytes));
         const uint32_t sa_addr = smem_u32(scales + s * (S::kSaBytes + S::kSbBytes)), sb_addr = sa_addr + S::kSaBytes;
         const uint64_t a_desc = smem_desc_sw128(a_addr), b_desc = smem_desc_sw128(a_addr + S::kABytes);
-        const uint32_t t_sa = tmem_base + BLOCK_N + (uint32_t)s * kScaleCols, t_sb = t_sa + 8;
+        const uint32_t t_sa = tmem_base + S::kScalesAt + (uint32_t)slot.at * S::kScaleCols, t_sb = t_sa + 8;
+        if (elect_one()) {
 #pragma unroll
-        for (int t = 0; t < 2; t++) {  // scale tiles: 128 elements of a row each
-          tmem_copy_scales(t_sa + 4 * t, smem_desc_rows16(sa_addr + 512 * t));
+          for (int h = 0; h < 2; h++) {  // scale tiles: 128 elements of a row each
+            tmem_copy_scales(t_sa + 4 * h, smem_desc_rows16(sa_addr + 512 * h));
 #pragma unroll
-          for (int r = 0; r < S::kRowTiles; r++)
-            tmem_copy_scales(t_sb + (uint32_t)(4 * (t * S::kRowTiles + r)), smem_desc_rows16(sb_addr + 1024 * r + 512 * t));
+            for (int r = 0; r < S::kRowTiles; r++)
+              tmem_copy_scales(t_sb + (uint32_t)(4 * (h * S::kRowTiles + r)), smem_desc_rows16(sb_addr + 1024 * r + 512 * h));
+          }
+          const int steps = min(4, p.k_steps - 4 * kb);
+#pragma unroll
+          for (int k = 0; k < 4; k++) {
+            const uint32_t id = (uint32_t)(k & 1) * 2;  // which two of a scale word's four bytes
+            if (k < steps)
+              umma_mxf4(d_tmem, a_desc + (uint64_t)(k * (kUmmaK >> 4)), b_desc + (uint64_t)(k * (kUmmaK >> 4)),
+                        idesc_mxf4(kBlockM, BLOCK_N) | id << 4 | id << 29, t_sa + 4 * (k >> 1),
+                        t_sb + (uint32_t)(4 * S::kRowTiles * (k >> 1) + (half_tile >> 5)), (kb | k) != 0);
+          }
+          umma_commit(&empty[s]);
         }
-#pragma unroll
-        for (int k = 0; k < 4; k++) {
-          const uint32_t id = (uint32_t)(k & 1) * 2;  // which two of a scale word's four bytes
-          umma_mxf4(tmem_base, a_desc + (uint64_t)(k * (kUmmaK >> 4)), b_desc + (uint64_t)(k * (kUmmaK >> 4)),
-                    idesc_mxf4(kBlockM, BLOCK_N) | id << 4 | id << 29, t_sa + 4 * (k >> 1),
-                    t_sb + (uint32_t)(4 * S::kRowTiles * (k >> 1)) + (BLOCK_N % 128 ? (uint32_t)((n0 & 127) >> 5) : 0u), (kb | k) != 0);
-        }
-        umma_commit(&empty[s]);
+        __syncwarp();
       }
-      if (live) umma_commit(acc_full);
+      if (live && elect_one()) umma_commit(&acc_full[buf]);
+      __syncwarp();
     }
   } else {
-    const int quarter = warp & 3;
-    const bool ok = __all_sync(0xffffffffu, mbar_wait(acc_full, 0, abort_flag));
-    if (ok) {
+    const int quarter = warp & 3, half = (warp - 2) >> 2, et = threadIdx.x - 64;
+    constexpr int kChunks = BLOCK_N / S::kChunk;
+    uint8_t *stage = staging + (warp - 2) * (32 * 128);  // 32 rows of 128 bytes, 16-byte pieces xor-ed with the row
+    int lt = 0;
+    bool dead = false;
+    for (int64_t t = blockIdx.x; t < tiles; t += gridDim.x, lt++) {
+      const int n_tile = (int)(t / m_tiles), m0 = (int)(t - (int64_t)n_tile * m_tiles) * kBlockM, n0 = n_tile * BLOCK_N;
+      const int buf = lt & 1;
+      float *tile_bias = bias + buf * BLOCK_N;
+      if (p.bias != nullptr) {
+        if (et < BLOCK_N) tile_bias[et] = n0 + et < p.N ? p.bias[n0 + et] : 0.0f;
+        asm volatile("bar.sync 1, %0;" ::"n"(kEpilogueWarps * 32) : "memory");
+      }
+      // A warp whose bounded wait gave up drains nothing any more, but walks on: the barrier counts every epilogue warp.
+      if (!dead) dead = !warp_wait(&acc_full[buf], (lt >> 1) & 1, abort_flag);
+      if (dead) continue;
       tc_fence_after();
-      const int row = m0 + quarter * 32 + lane;
-      const uint32_t lane_addr = tmem_base + ((uint32_t)(quarter * 32) << 16);
-      Out *out = reinterpret_cast<Out *>(p.out) + (size_t)row * p.N;
+      const uint32_t lane_addr = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(buf * (BLOCK_N - S::kShared));
+      // chunks whose draining frees what the next tile waits for: the shared columns, else all
+      constexpr int kFirst = S::kShared ? S::kShared / S::kChunk : kChunks;
+      const int last_of_first = kFirst - 1 < half ? -1 : (kFirst - 1 - half) / 2 * 2 + half;
+      if (last_of_first < 0 && lane == 0) mbar_arrive(&acc_empty[buf]);
 #pragma unroll 1
-      for (int c = 0; c < BLOCK_N; c += 16) {
-        uint32_t acc[16];
-        tmem_ld_32x32b_x16(lane_addr + (uint32_t)c, acc);
-        tmem_ld_wait();
+      for (int i = half; i < kChunks; i += 2) {
+        const int c = (S::kShared && buf == 0 ? kChunks - 1 - i : i) * S::kChunk;  // (the first accumulator shares its last columns)
+        uint32_t acc[S::kChunk];
 #pragma unroll
-        for (int i = 0; i < 16; i++) {
-          const int j = n0 + c + i;
-          if (row < p.M && j < p.N) {
-            float v = __uint_as_float(acc[i]);
-            if (p.bias) v += __ldg(p.bias + j);
-            if (p.relu) v = v < 0.0f ? 0.0f : v;
-            out[j] = from_float<Out>(v);
+        for (int q = 0; q < S::kChunk; q += 16) tmem_ld_32x32b_x16(lane_addr + (uint32_t)(c + q), *reinterpret_cast<uint32_t(*)[16]>(acc + q));
+        tmem_ld_wait();
+        if (i == last_of_first) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&acc_empty[buf]);
+        }
+        if (n0 + c >= p.N) continue;
+        if (p.bias != nullptr) {
+#pragma unroll
+          for (int q = 0; q < S::kChunk; q += 4) {
+            const float4 b = *reinterpret_cast<const float4 *>(tile_bias + c + q);
+            acc[q] = __float_as_uint(__uint_as_float(acc[q]) + b.x);
+            acc[q + 1] = __float_as_uint(__uint_as_float(acc[q + 1]) + b.y);
+            acc[q + 2] = __float_as_uint(__uint_as_float(acc[q + 2]) + b.z);
+            acc[q + 3] = __float_as_uint(__uint_as_float(acc[q + 3]) + b.w);
           }
         }
+        if (p.relu) {
+#pragma unroll
+          for (int q = 0; q < S::kChunk; q++) acc[q] = __uint_as_float(acc[q]) < 0.0f ? 0u : acc[q];
+        }
+        if (p.store_by_tma && lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+        __syncwarp();  // the staging area is free again
+#pragma unroll
+        for (int q = 0; q < 8; q++) {
+          uint4 w;
+          if constexpr (sizeof(Out) == 4) {
+            w = make_uint4(acc[4 * q], acc[4 * q + 1], acc[4 * q + 2], acc[4 * q + 3]);
+          } else {
+            uint32_t h[4];
+#pragma unroll
+            for (int e = 0; e < 4; e++) h[e] = pack2(__uint_as_float(acc[8 * q + 2 * e]), __uint_as_float(acc[8 * q + 2 * e + 1]), Out());
+            w = make_uint4(h[0], h[1], h[2], h[3]);
+          }
+          *reinterpret_cast<uint4 *>(stage + lane * 128 + 16 * (q ^ (lane & 7))) = w;
+        }
+        if (p.store_by_tma) {
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          __syncwarp();
+          if (lane == 0 && m0 + quarter * 32 < p.M) {
+            tma_store_2d(&map_out, stage, n0 + c, m0 + quarter * 32);
+            asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+          }
+        } else {  // rows off 16-byte boundaries
+          __syncwarp();
+          const int rows = min(32, p.M - m0 - quarter * 32), cols = min(S::kChunk, p.N - n0 - c);
+          Out *out = reinterpret_cast<Out *>(p.out) + (size_t)(m0 + quarter * 32) * p.N + n0 + c;
+          for (int r = 0; r < rows; r++)
+            for (int j = lane; j < cols; j += 32)
+              out[(size_t)r * p.N + j] = *reinterpret_cast<const Out *>(stage + r * 128 + ((j * (int)sizeof(Out)) ^ (16 * (r & 7))));
+        }
       }
-    } else if (lane == 0 && p.status != nullptr) {
-      atomicOr(p.status, GLOWB200_STATUS_WAIT_TIMEOUT);
     }
+    if (p.store_by_tma && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+    if (dead && lane == 0 && p.status != nullptr) atomicOr(p.status, GLOWB200_STATUS_WAIT_TIMEOUT);
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == 1) tmem_dealloc(tmem_base, kTmemCols);
+  if (warp == 1) tmem_dealloc(tmem_base, 512);
 }
 
 // [rows, pitch] bytes, box of 128 bytes by box_rows, 128-byte swizzle.
@@ -180,6 +327,18 @@ int make_data_map(CUtensorMap *map, const void *base, int64_t rows, int64_t pitc
   cuuint32_t box[2] = {(cuuint32_t)kBlockK, (cuuint32_t)box_rows}, estr[2] = {1, 1};
   CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void *>(base), dims, strides, box, estr,
                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return set_error(GLOWB200_ERR_CUDA, "cuTensorMapEncodeTiled failed with CUresult %d", (int)r);
+  return GLOWB200_OK;
+}
+// the result [M, N]: boxes of 32 rows by 128 bytes, in the 128-byte swizzle
+int make_out_map(CUtensorMap *map, const FcParams &p, int bytes) {
+  EncodeTiledFn fn = encode_tiled_fn();
+  if (!fn) return set_error(GLOWB200_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
+  cuuint64_t dims[2] = {(cuuint64_t)p.N, (cuuint64_t)p.M}, strides[1] = {(cuuint64_t)p.N * bytes};
+  cuuint32_t box[2] = {(cuuint32_t)(128 / bytes), 32}, estr[2] = {1, 1};
+  CUresult r = fn(map, bytes == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, p.out, dims, strides, box, estr,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_NONE,
                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return set_error(GLOWB200_ERR_CUDA, "cuTensorMapEncodeTiled failed with CUresult %d", (int)r);
   return GLOWB200_OK;
@@ -198,18 +357,31 @@ int make_scale_map(CUtensorMap *map, const void *base, int64_t row_tiles, int64_
 }
 
 template <int BLOCK_N, int STAGES, typename Out>
-int launch(const void *a, const void *sa, const void *b, const void *sb, int64_t K, const FcParams &p, cudaStream_t s) {
-  using S = Smem<BLOCK_N, STAGES>;
+int launch_tiles(const void *a, const void *sa, const void *b, const void *sb, int64_t K, FcParams p, cudaStream_t s) {
+  using S = Tile<BLOCK_N, STAGES, Out>;
   const int64_t pitch = mx_pitch(K), tiles = mx_tiles(K);
-  CUtensorMap ma, mb, msa, msb;
+  CUtensorMap ma, mb, msa, msb, mout = {};
   if (int rc = make_data_map(&ma, a, p.M, pitch, kBlockM)) return rc;
   if (int rc = make_data_map(&mb, b, p.N, pitch, BLOCK_N)) return rc;
   if (int rc = make_scale_map(&msa, sa, mx_row_tiles(p.M), tiles, 1)) return rc;
   if (int rc = make_scale_map(&msb, sb, mx_row_tiles(p.N), tiles, S::kRowTiles)) return rc;
+  p.store_by_tma = aligned(p.out, 16) && (int64_t)p.N * sizeof(Out) % 16 == 0;
+  if (p.store_by_tma)
+    if (int rc = make_out_map(&mout, p, sizeof(Out))) return rc;
   auto kernel = fp4_gemm_kernel<BLOCK_N, STAGES, Out>;
   GLOWB200_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kTotal));
-  GLOWB200_CUDA_OK(launch_pdl(kernel, dim3((p.M + kBlockM - 1) / kBlockM, (p.N + BLOCK_N - 1) / BLOCK_N), kThreads, S::kTotal, s, ma, mb, msa, msb, p));
+  const int64_t blocks = (int64_t)((p.M + kBlockM - 1) / kBlockM) * ((p.N + BLOCK_N - 1) / BLOCK_N), sms = sm_count();
+  GLOWB200_CUDA_OK(launch_pdl(kernel, dim3((unsigned)(blocks < sms ? blocks : sms)), kThreads, S::kTotal, s, ma, mb, msa, msb, mout, p));
   return GLOWB200_OK;
+}
+
+template <typename Out>
+int launch(const void *a, const void *sa, const void *b, const void *sb, int64_t K, const FcParams &p, cudaStream_t s) {
+  const int64_t m_tiles = (p.M + kBlockM - 1) / kBlockM, sms = sm_count();
+  auto rounds = [&](int n) { return ((m_tiles * ((p.N + n - 1) / n) + sms - 1) / sms) * n; };
+  if (rounds(256) <= rounds(128) && rounds(256) <= rounds(64)) return launch_tiles<256, 3, Out>(a, sa, b, sb, K, p, s);
+  if (rounds(128) <= rounds(64)) return launch_tiles<128, 5, Out>(a, sa, b, sb, K, p, s);
+  return launch_tiles<64, 7, Out>(a, sa, b, sb, K, p, s);
 }
 
 int check_fc(const void *out, int out_type, const void *in, const void *weights, const void *weights_scales, int64_t M, int64_t K, int64_t N, int flags) {
@@ -225,9 +397,9 @@ int check_fc(const void *out, int out_type, const void *in, const void *weights,
 
 int run_fc(void *out, int out_type, const void *a, const void *sa, const void *b, const void *sb, const float *bias, int64_t M, int64_t K,
            int64_t N, int flags, int32_t *status, cudaStream_t s) {
-  const FcParams p{out, bias, status, (int)M, (int)N, (int)((K + 63) / 64), (flags & GLOWB200_FC_FUSE_RELU) != 0};
+  const FcParams p{out, bias, status, (int)M, (int)N, (int)((K + 63) / 64), (flags & GLOWB200_FC_FUSE_RELU) != 0, 0};
   return with_float_type(out_type, [&](auto *t) {
-    return launch<256, 4, std::remove_pointer_t<decltype(t)>>(a, sa, b, sb, K, p, s);
+    return launch<std::remove_pointer_t<decltype(t)>>(a, sa, b, sb, K, p, s);
   });
 }
 
