@@ -60,11 +60,10 @@ struct Tile {
   static constexpr int kStaging = kEpilogueWarps * 32 * 128;
   static constexpr int kTotal = STAGES * kStageBytes + kStaging + 2 * BLOCK_N * 4 + 256 + 1024;
   static_assert(kTotal <= 232448, "more shared memory than a CTA can have");
-  static constexpr int kShared = BLOCK_N == 256 ? 64 : 0;
+  static constexpr int kShared = BLOCK_N == 256 ? 128 : 0;
   static constexpr uint32_t kScaleCols = 8 + 8 * kRowTiles;  // of one k-block
   static constexpr uint32_t kScalesAt = 2 * BLOCK_N - kShared;
-  static constexpr int kSlots = BLOCK_N == 256 ? 2 : 4;
-  static_assert(kScalesAt + kSlots * kScaleCols <= 512 && kSlots <= STAGES && kShared % kChunk == 0, "tensor memory");
+  static_assert(kScalesAt + STAGES * kScaleCols <= 512 && kShared % kChunk == 0, "tensor memory");
 };
 
 __device__ __forceinline__ uint32_t pack2(float lo, float hi, __half) {
@@ -177,9 +176,7 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
       }
     }
   } else if (warp == 1) {
-    Ring<STAGES> ring, done;  // done: the k-block whose MMAs have to be complete before its scales' columns are taken again
-    Ring<S::kSlots> slot;
-    int started = 0;
+    Ring<STAGES> ring;
     int lt = 0;
     bool live = true;
     for (int64_t t = blockIdx.x; t < tiles && live; t += gridDim.x, lt++) {
@@ -190,20 +187,18 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
                      : lt >= 2 && !warp_wait(&acc_empty[buf], ((lt >> 1) - 1) & 1, abort_flag)) break;
       tc_fence_after();
       const uint32_t d_tmem = tmem_base + (uint32_t)(buf * (BLOCK_N - S::kShared));
-      for (int kb = 0; kb < k_blocks; kb++, ring.next(), slot.next()) {
+      // The scales of a stage have columns of their own: a stage that is full again was empty, so the MMAs that read them are done.
+      bool ready = mbar_try_wait(&full[ring.at], ring.round);
+      for (int kb = 0; kb < k_blocks; kb++) {
         const int s = ring.at;
-        if (!warp_wait(&full[s], ring.round, abort_flag)) { live = false; break; }
-        if (started < S::kSlots) {
-          started++;
-        } else {
-          if (!warp_wait(&empty[done.at], done.round, abort_flag)) { live = false; break; }
-          done.next();
-        }
+        if (!__all_sync(0xffffffffu, ready) && !warp_wait(&full[s], ring.round, abort_flag)) { live = false; break; }
         tc_fence_after();
+        ring.next();
+        ready = kb + 1 < k_blocks && mbar_try_wait(&full[ring.at], ring.round);  // (asked before this k-block's MMAs are issued)
         const uint32_t a_addr = smem_u32(smem + s * (S::kABytes + S::kBBytes));
         const uint32_t sa_addr = smem_u32(scales + s * (S::kSaBytes + S::kSbBytes)), sb_addr = sa_addr + S::kSaBytes;
         const uint64_t a_desc = smem_desc_sw128(a_addr), b_desc = smem_desc_sw128(a_addr + S::kABytes);
-        const uint32_t t_sa = tmem_base + S::kScalesAt + (uint32_t)slot.at * S::kScaleCols, t_sb = t_sa + 8;
+        const uint32_t t_sa = tmem_base + S::kScalesAt + (uint32_t)s * S::kScaleCols, t_sb = t_sa + 8;
         if (elect_one()) {
 #pragma unroll
           for (int h = 0; h < 2; h++) {  // scale tiles: 128 elements of a row each
