@@ -17,18 +17,37 @@ constexpr int kUmmaK = 32;    // bytes of a row per MMA: 64 elements, two scales
 constexpr int kEpilogueWarps = 8;  // two to a lane quarter of tensor memory
 constexpr int kThreads = 64 + 32 * kEpilogueWarps;
 
+// PAIR: one MMA over the two SMs of a cluster of two blocks, 256 rows: each has its own 128 rows of A and of the
+// result, its own scales and half of B's rows.
+template <bool PAIR>
 __device__ __forceinline__ void umma_mxf4(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t a_scales,
                                           uint32_t b_scales, uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %6, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
-      ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(a_scales), "r"(b_scales), "r"(accumulate)
-      : "memory");
+  if constexpr (PAIR)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
+        ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(a_scales), "r"(b_scales), "r"(accumulate)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
+        ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(a_scales), "r"(b_scales), "r"(accumulate)
+        : "memory");
 }
-// 512 bytes of scales -> four columns of tensor memory, in each of the four lane quarters.
+// 512 bytes of scales -> four columns of tensor memory, in each of the four lane quarters (PAIR: in both blocks, each
+// from its own shared memory).
+template <bool PAIR>
 __device__ __forceinline__ void tmem_copy_scales(uint32_t taddr, uint64_t desc) {
-  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+  if constexpr (PAIR) asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+  else asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+}
+// Arrives on a barrier of another block of the cluster, for that block's tensor core to go on: what it waits for has been
+// read into registers, no memory is handed over, and a release to the cluster would take a thousand clocks.
+__device__ __forceinline__ void mbar_arrive_remote(uint32_t cluster_addr) {
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
 // Descriptor of 32 rows of 16 bytes, one behind the other (no swizzle): 8-row groups are 128 bytes apart.
 __device__ __forceinline__ uint64_t smem_desc_rows16(uint32_t smem_addr) {
@@ -50,10 +69,12 @@ struct FcParams {
 // Tensor memory (512 columns): two accumulators, then the scales of the k-blocks in flight.  Two accumulators of 256
 // columns would leave no room for the scales, so they share kShared columns there: the epilogue empties those first, and
 // the next tile's MMAs start as soon as it has.
-template <int BLOCK_N, int STAGES, typename Out>
+template <int BLOCK_N, int STAGES, bool PAIR, typename Out>
 struct Tile {
+  static constexpr int kRows = PAIR ? 2 * kBlockM : kBlockM;  // of a tile
   static constexpr int kRowTiles = (BLOCK_N + 127) / 128;  // of the right operand's scales
-  static constexpr int kABytes = kBlockM * kBlockK, kBBytes = BLOCK_N * kBlockK;
+  static constexpr int kBRows = PAIR ? BLOCK_N / 2 : BLOCK_N;  // that a block loads
+  static constexpr int kABytes = kBlockM * kBlockK, kBBytes = kBRows * kBlockK;
   static constexpr int kSaBytes = 1024, kSbBytes = 1024 * kRowTiles;
   static constexpr int kStageBytes = kABytes + kBBytes + kSaBytes + kSbBytes;
   static constexpr int kChunk = 128 / (int)sizeof(Out);  // columns that a warp drains at a time: rows of 128 bytes
@@ -109,14 +130,15 @@ struct Ring {
   }
 };
 
-// Persistent: blocks walk the 128 x BLOCK_N tiles, row tile fastest (blocks that run together share weights).  Warp 0
-// loads, warp 1 issues the copies of the scales and the MMAs, warps 2 to 9 drain.
-template <int BLOCK_N, int STAGES, typename Out>
+// Persistent: blocks, or pairs of them, walk the 128 x BLOCK_N (256 x BLOCK_N) tiles, row tile fastest (blocks that run
+// together share weights).  Warp 0 loads, warp 1 (of a pair's even block) issues the copies of the scales and the MMAs,
+// warps 2 to 9 drain.  The loads of a pair's two blocks are counted on the even one's barrier.
+template <int BLOCK_N, int STAGES, bool PAIR, typename Out>
 __global__ void __launch_bounds__(kThreads, 1)
 fp4_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                 const __grid_constant__ CUtensorMap map_sa, const __grid_constant__ CUtensorMap map_sb,
                 const __grid_constant__ CUtensorMap map_out, const FcParams p) {
-  using S = Tile<BLOCK_N, STAGES, Out>;
+  using S = Tile<BLOCK_N, STAGES, PAIR, Out>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   uint8_t *staging = smem + STAGES * (S::kABytes + S::kBBytes);
@@ -137,40 +159,57 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
     }
     for (int b = 0; b < 2; b++) {
       mbar_init(&acc_full[b], 1);
-      mbar_init(&acc_empty[b], kEpilogueWarps);
+      mbar_init(&acc_empty[b], (PAIR ? 2 : 1) * kEpilogueWarps);
     }
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 1) {
-    tmem_alloc(tmem_slot, 512);
-    tmem_relinquish();
+    if constexpr (PAIR) {
+      tmem_alloc_pair(tmem_slot, 512);
+      tmem_relinquish_pair();
+    } else {
+      tmem_alloc(tmem_slot, 512);
+      tmem_relinquish();
+    }
   }
   tc_fence_before();
   __syncthreads();
+  if constexpr (PAIR) cluster_sync();  // the partner's barriers exist before anything signals them
   tc_fence_after();
   pdl_wait();
   pdl_launch_dependents();
   const uint32_t tmem_base = __shfl_sync(0xffffffffu, *tmem_slot, 0);
-  const int m_tiles = (p.M + kBlockM - 1) / kBlockM, n_tiles = (p.N + BLOCK_N - 1) / BLOCK_N;
+  const int rank = PAIR ? (int)cluster_ctarank() : 0;
+  const int64_t walker = PAIR ? blockIdx.x >> 1 : blockIdx.x, walkers = PAIR ? gridDim.x >> 1 : gridDim.x;
+  const int m_tiles = (p.M + S::kRows - 1) / S::kRows, n_tiles = (p.N + BLOCK_N - 1) / BLOCK_N;
   const int64_t tiles = (int64_t)m_tiles * n_tiles;
   const int k_blocks = (p.k_steps + 3) >> 2;
 
   if (warp == 0) {
     Ring<STAGES> ring;
     bool live = true;
-    for (int64_t t = blockIdx.x; t < tiles && live; t += gridDim.x) {
-      const int n_tile = (int)(t / m_tiles), m0 = (int)(t - (int64_t)n_tile * m_tiles) * kBlockM, n0 = n_tile * BLOCK_N;
+    for (int64_t t = walker; t < tiles && live; t += walkers) {
+      const int n_tile = (int)(t / m_tiles), m0 = (int)(t - (int64_t)n_tile * m_tiles) * S::kRows + rank * kBlockM, n0 = n_tile * BLOCK_N;
       for (int kb = 0; kb < k_blocks; kb++, ring.next()) {
         const int s = ring.at;
         if (!warp_wait(&empty[s], ring.round ^ 1, abort_flag)) { live = false; break; }  // (passes at once the first time round)
         uint8_t *a = smem + s * (S::kABytes + S::kBBytes), *sa = scales + s * (S::kSaBytes + S::kSbBytes);
         if (elect_one()) {
-          mbar_expect_tx(&full[s], S::kStageBytes);
-          tma_load_2d(sa, &map_sa, kb * 256, m0 >> 7, &full[s]);
-          tma_load_2d(sa + S::kSaBytes, &map_sb, kb * 256, n0 >> 7, &full[s]);
-          tma_load_2d(a, &map_a, kb * kBlockK, m0, &full[s]);
-          tma_load_2d(a + S::kABytes, &map_b, kb * kBlockK, n0, &full[s]);
+          if constexpr (PAIR) {
+            if (rank == 0) mbar_expect_tx(&full[s], 2 * S::kStageBytes);
+            const uint32_t counted = map_to_cta(&full[s], 0);
+            tma_load_2d_pair(sa, &map_sa, kb * 256, m0 >> 7, counted);
+            tma_load_2d_pair(sa + S::kSaBytes, &map_sb, kb * 256, n0 >> 7, counted);
+            tma_load_2d_pair(a, &map_a, kb * kBlockK, m0, counted);
+            tma_load_2d_pair(a + S::kABytes, &map_b, kb * kBlockK, n0 + rank * S::kBRows, counted);
+          } else {
+            mbar_expect_tx(&full[s], S::kStageBytes);
+            tma_load_2d(sa, &map_sa, kb * 256, m0 >> 7, &full[s]);
+            tma_load_2d(sa + S::kSaBytes, &map_sb, kb * 256, n0 >> 7, &full[s]);
+            tma_load_2d(a, &map_a, kb * kBlockK, m0, &full[s]);
+            tma_load_2d(a + S::kABytes, &map_b, kb * kBlockK, n0, &full[s]);
+          }
         }
         __syncwarp();
       }
@@ -178,8 +217,8 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
   } else if (warp == 1) {
     Ring<STAGES> ring;
     int lt = 0;
-    bool live = true;
-    for (int64_t t = blockIdx.x; t < tiles && live; t += gridDim.x, lt++) {
+    bool live = rank == 0;
+    for (int64_t t = walker; t < tiles && live; t += walkers, lt++) {
       const int buf = lt & 1;
       const int half_tile = BLOCK_N % 128 ? (int)(t / m_tiles) * BLOCK_N & 127 : 0;  // rows of the first scale tile in front of this tile's
       // The columns this tile's sums go to: of the shared ones the tile before has to be gone, else the one before that.
@@ -202,35 +241,44 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
         if (elect_one()) {
 #pragma unroll
           for (int h = 0; h < 2; h++) {  // scale tiles: 128 elements of a row each
-            tmem_copy_scales(t_sa + 4 * h, smem_desc_rows16(sa_addr + 512 * h));
+            tmem_copy_scales<PAIR>(t_sa + 4 * h, smem_desc_rows16(sa_addr + 512 * h));
 #pragma unroll
             for (int r = 0; r < S::kRowTiles; r++)
-              tmem_copy_scales(t_sb + (uint32_t)(4 * (h * S::kRowTiles + r)), smem_desc_rows16(sb_addr + 1024 * r + 512 * h));
+              tmem_copy_scales<PAIR>(t_sb + (uint32_t)(4 * (h * S::kRowTiles + r)), smem_desc_rows16(sb_addr + 1024 * r + 512 * h));
           }
           const int steps = min(4, p.k_steps - 4 * kb);
 #pragma unroll
           for (int k = 0; k < 4; k++) {
             const uint32_t id = (uint32_t)(k & 1) * 2;  // which two of a scale word's four bytes
             if (k < steps)
-              umma_mxf4(d_tmem, a_desc + (uint64_t)(k * (kUmmaK >> 4)), b_desc + (uint64_t)(k * (kUmmaK >> 4)),
-                        idesc_mxf4(kBlockM, BLOCK_N) | id << 4 | id << 29, t_sa + 4 * (k >> 1),
+              umma_mxf4<PAIR>(d_tmem, a_desc + (uint64_t)(k * (kUmmaK >> 4)), b_desc + (uint64_t)(k * (kUmmaK >> 4)),
+                        idesc_mxf4(S::kRows, BLOCK_N) | id << 4 | id << 29, t_sa + 4 * (k >> 1),
                         t_sb + (uint32_t)(4 * S::kRowTiles * (k >> 1) + (half_tile >> 5)), (kb | k) != 0);
           }
-          umma_commit(&empty[s]);
+          if constexpr (PAIR) umma_commit_pair(&empty[s]);
+          else umma_commit(&empty[s]);
         }
         __syncwarp();
       }
-      if (live && elect_one()) umma_commit(&acc_full[buf]);
+      if (live && elect_one()) {
+        if constexpr (PAIR) umma_commit_pair(&acc_full[buf]);
+        else umma_commit(&acc_full[buf]);
+      }
       __syncwarp();
     }
   } else {
     const int quarter = warp & 3, half = (warp - 2) >> 2, et = threadIdx.x - 64;
     constexpr int kChunks = BLOCK_N / S::kChunk;
     uint8_t *stage = staging + (warp - 2) * (32 * 128);  // 32 rows of 128 bytes, 16-byte pieces xor-ed with the row
+    const uint32_t drained = PAIR ? map_to_cta(acc_empty, 0) : 0u;
+    auto arrive_drained = [&](int buf) {
+      if constexpr (PAIR) mbar_arrive_remote(drained + 8 * buf);
+      else mbar_arrive(&acc_empty[buf]);
+    };
     int lt = 0;
     bool dead = false;
-    for (int64_t t = blockIdx.x; t < tiles; t += gridDim.x, lt++) {
-      const int n_tile = (int)(t / m_tiles), m0 = (int)(t - (int64_t)n_tile * m_tiles) * kBlockM, n0 = n_tile * BLOCK_N;
+    for (int64_t t = walker; t < tiles; t += walkers, lt++) {
+      const int n_tile = (int)(t / m_tiles), m0 = (int)(t - (int64_t)n_tile * m_tiles) * S::kRows + rank * kBlockM, n0 = n_tile * BLOCK_N;
       const int buf = lt & 1;
       float *tile_bias = bias + buf * BLOCK_N;
       if (p.bias != nullptr) {
@@ -245,7 +293,7 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
       // chunks whose draining frees what the next tile waits for: the shared columns, else all
       constexpr int kFirst = S::kShared ? S::kShared / S::kChunk : kChunks;
       const int last_of_first = kFirst - 1 < half ? -1 : (kFirst - 1 - half) / 2 * 2 + half;
-      if (last_of_first < 0 && lane == 0) mbar_arrive(&acc_empty[buf]);
+      if (last_of_first < 0 && lane == 0) arrive_drained(buf);
 #pragma unroll 1
       for (int i = half; i < kChunks; i += 2) {
         const int c = (S::kShared && buf == 0 ? kChunks - 1 - i : i) * S::kChunk;  // (the first accumulator shares its last columns)
@@ -256,7 +304,7 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
         if (i == last_of_first) {
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive(&acc_empty[buf]);
+          if (lane == 0) arrive_drained(buf);
         }
         if (n0 + c >= p.N) continue;
         if (p.bias != nullptr) {
@@ -306,12 +354,22 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
       }
     }
     if (p.store_by_tma && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
-    if (dead && lane == 0 && p.status != nullptr) atomicOr(p.status, GLOWB200_STATUS_WAIT_TIMEOUT);
   }
   tc_fence_before();
   __syncthreads();
+  if (*abort_flag) {  // a wait gave up: copies that are still on their way here get a bounded time to land
+    if (threadIdx.x == 0 && p.status != nullptr) atomicOr(p.status, GLOWB200_STATUS_WAIT_TIMEOUT);
+    const long long t0 = clock64();
+    while (clock64() - t0 < 4000000ll) {
+    }
+    __syncthreads();
+  }
+  if constexpr (PAIR) cluster_sync();  // neither block leaves while its partner may read its tiles
   tc_fence_after();
-  if (warp == 1) tmem_dealloc(tmem_base, 512);
+  if (warp == 1) {
+    if constexpr (PAIR) tmem_dealloc_pair(tmem_base, 512);
+    else tmem_dealloc(tmem_base, 512);
+  }
 }
 
 // [rows, pitch] bytes, box of 128 bytes by box_rows, 128-byte swizzle.
@@ -351,32 +409,70 @@ int make_scale_map(CUtensorMap *map, const void *base, int64_t row_tiles, int64_
   return GLOWB200_OK;
 }
 
-template <int BLOCK_N, int STAGES, typename Out>
+template <int BLOCK_N, int STAGES, bool PAIR, typename Out>
 int launch_tiles(const void *a, const void *sa, const void *b, const void *sb, int64_t K, FcParams p, cudaStream_t s) {
-  using S = Tile<BLOCK_N, STAGES, Out>;
+  using S = Tile<BLOCK_N, STAGES, PAIR, Out>;
   const int64_t pitch = mx_pitch(K), tiles = mx_tiles(K);
   CUtensorMap ma, mb, msa, msb, mout = {};
   if (int rc = make_data_map(&ma, a, p.M, pitch, kBlockM)) return rc;
-  if (int rc = make_data_map(&mb, b, p.N, pitch, BLOCK_N)) return rc;
+  if (int rc = make_data_map(&mb, b, p.N, pitch, S::kBRows)) return rc;
   if (int rc = make_scale_map(&msa, sa, mx_row_tiles(p.M), tiles, 1)) return rc;
   if (int rc = make_scale_map(&msb, sb, mx_row_tiles(p.N), tiles, S::kRowTiles)) return rc;
   p.store_by_tma = aligned(p.out, 16) && (int64_t)p.N * sizeof(Out) % 16 == 0;
   if (p.store_by_tma)
     if (int rc = make_out_map(&mout, p, sizeof(Out))) return rc;
-  auto kernel = fp4_gemm_kernel<BLOCK_N, STAGES, Out>;
+  auto kernel = fp4_gemm_kernel<BLOCK_N, STAGES, PAIR, Out>;
   GLOWB200_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kTotal));
-  const int64_t blocks = (int64_t)((p.M + kBlockM - 1) / kBlockM) * ((p.N + BLOCK_N - 1) / BLOCK_N), sms = sm_count();
-  GLOWB200_CUDA_OK(launch_pdl(kernel, dim3((unsigned)(blocks < sms ? blocks : sms)), kThreads, S::kTotal, s, ma, mb, msa, msb, mout, p));
+  const int64_t work = (int64_t)((p.M + S::kRows - 1) / S::kRows) * ((p.N + BLOCK_N - 1) / BLOCK_N), most = sm_count() / (PAIR ? 2 : 1);
+  const int64_t walkers = work < most ? work : most;
+  if constexpr (!PAIR) {
+    GLOWB200_CUDA_OK(launch_pdl(kernel, dim3((unsigned)walkers), kThreads, S::kTotal, s, ma, mb, msa, msb, mout, p));
+  } else {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(2 * walkers));
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = S::kTotal;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 2;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = pdl_enabled() ? 2 : 1;
+    GLOWB200_CUDA_OK(cudaLaunchKernelEx(&cfg, kernel, ma, mb, msa, msb, mout, static_cast<const FcParams>(p)));
+  }
   return GLOWB200_OK;
 }
 
 template <typename Out>
 int launch(const void *a, const void *sa, const void *b, const void *sb, int64_t K, const FcParams &p, cudaStream_t s) {
-  const int64_t m_tiles = (p.M + kBlockM - 1) / kBlockM, sms = sm_count();
-  auto rounds = [&](int n) { return ((m_tiles * ((p.N + n - 1) / n) + sms - 1) / sms) * n; };
-  if (rounds(256) <= rounds(128) && rounds(256) <= rounds(64)) return launch_tiles<256, 3, Out>(a, sa, b, sb, K, p, s);
-  if (rounds(128) <= rounds(64)) return launch_tiles<128, 5, Out>(a, sa, b, sb, K, p, s);
-  return launch_tiles<64, 7, Out>(a, sa, b, sb, K, p, s);
+  // The tile whose rounds over the SMs take least: measured microseconds of a k-block and of what a tile costs beside its
+  // k-blocks.  2048 x 4096 x 4096 takes 15.7 us in 256 x 256 tiles of pairs, 16.6 in 128 x 256, 22.3 in 128 x 128, 33 in
+  // 128 x 64; 512 x 4096 x 4096 9.1, 9.1, 7.9, 11.2; 128 x 4096 x 37888 17.2, 13.8, 14.3, 20.4; 128 x 4096 x 256 8.4, 8.7, 7.0, 6.4.
+  struct Kind {
+    int rows, cols, sms;
+    float block, tile;
+  };
+  constexpr Kind kKinds[4] = {{256, 256, 2, 0.33f, 1.6f}, {128, 256, 1, 0.37f, 1.7f}, {128, 128, 1, 0.265f, 0.9f}, {128, 64, 1, 0.235f, 0.5f}};
+  int best = 0;
+  float least = 0.0f;
+  for (int i = 0; i < 4; i++) {
+    const Kind &k = kKinds[i];
+    const int64_t tiles = (int64_t)((p.M + k.rows - 1) / k.rows) * ((p.N + k.cols - 1) / k.cols), at_once = sm_count() / k.sms;
+    const float cost = (float)((tiles + at_once - 1) / at_once) * ((float)((p.k_steps + 3) / 4) * k.block + k.tile);
+    if (i == 0 || cost < least) {
+      best = i;
+      least = cost;
+    }
+  }
+  switch (best) {
+    case 0: return launch_tiles<256, 5, true, Out>(a, sa, b, sb, K, p, s);
+    case 1: return launch_tiles<256, 3, false, Out>(a, sa, b, sb, K, p, s);
+    case 2: return launch_tiles<128, 5, false, Out>(a, sa, b, sb, K, p, s);
+    default: return launch_tiles<64, 7, false, Out>(a, sa, b, sb, K, p, s);
+  }
 }
 
 int check_fc(const void *out, int out_type, const void *in, const void *weights, const void *weights_scales, int64_t M, int64_t K, int64_t N, int flags) {
