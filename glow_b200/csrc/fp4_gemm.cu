@@ -5,67 +5,43 @@
 // A and B hold E2M1 numbers, two to a byte, with an E8M0 scale per 32 neighbours of a row, in the layout that
 // microscaled.cu writes.  The MMA takes the scales itself (tcgen05.mma kind::mxf4, one scale per 32 elements), its
 // products of two 4-bit numbers and two powers of two are exact, and the sums are fp32 in tensor memory.
-#include "microscaled.cuh"
-#include "tcgen05.cuh"
+#include "fp4_mma.cuh"
 
 namespace glowb200 {
+
+int make_data_map(CUtensorMap *map, const void *base, int64_t rows, int64_t pitch, int box_rows) {
+  EncodeTiledFn fn = encode_tiled_fn();
+  if (!fn) return set_error(GLOWB200_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
+  cuuint64_t dims[2] = {(cuuint64_t)pitch, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)pitch};
+  cuuint32_t box[2] = {(cuuint32_t)kBlockK, (cuuint32_t)box_rows}, estr[2] = {1, 1};
+  CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void *>(base), dims, strides, box, estr,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return set_error(GLOWB200_ERR_CUDA, "cuTensorMapEncodeTiled failed with CUresult %d", (int)r);
+  return GLOWB200_OK;
+}
+int make_scale_map(CUtensorMap *map, const void *base, int64_t row_tiles, int64_t tiles, int box_tiles) {
+  EncodeTiledFn fn = encode_tiled_fn();
+  if (!fn) return set_error(GLOWB200_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
+  cuuint64_t dims[2] = {(cuuint64_t)tiles * 128, (cuuint64_t)row_tiles}, strides[1] = {(cuuint64_t)tiles * 512};
+  cuuint32_t box[2] = {256, (cuuint32_t)box_tiles}, estr[2] = {1, 1};
+  CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT32, 2, const_cast<void *>(base), dims, strides, box, estr,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return set_error(GLOWB200_ERR_CUDA, "cuTensorMapEncodeTiled failed with CUresult %d", (int)r);
+  return GLOWB200_OK;
+}
+
 namespace {
 
-constexpr int kBlockM = 128;
-constexpr int kBlockK = 128;  // bytes of a row per pipeline stage: 256 elements, one 128-byte swizzle atom
-constexpr int kUmmaK = 32;    // bytes of a row per MMA: 64 elements, two scales
 constexpr int kEpilogueWarps = 8;  // two to a lane quarter of tensor memory
 constexpr int kThreads = 64 + 32 * kEpilogueWarps;
 
-// PAIR: one MMA over the two SMs of a cluster of two blocks, 256 rows: each has its own 128 rows of A and of the
-// result, its own scales and half of B's rows.
-template <bool PAIR>
-__device__ __forceinline__ void umma_mxf4(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t a_scales,
-                                          uint32_t b_scales, uint32_t accumulate) {
-  if constexpr (PAIR)
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %6, 0;\n\t"
-        "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
-        ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(a_scales), "r"(b_scales), "r"(accumulate)
-        : "memory");
-  else
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %6, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
-        ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(a_scales), "r"(b_scales), "r"(accumulate)
-        : "memory");
-}
-// 512 bytes of scales -> four columns of tensor memory, in each of the four lane quarters (PAIR: in both blocks, each
-// from its own shared memory).
-template <bool PAIR>
-__device__ __forceinline__ void tmem_copy_scales(uint32_t taddr, uint64_t desc) {
-  if constexpr (PAIR) asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
-  else asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
-}
 // Arrives on a barrier of another block of the cluster, for that block's tensor core to go on: what it waits for has been
 // read into registers, no memory is handed over, and a release to the cluster would take a thousand clocks.
 __device__ __forceinline__ void mbar_arrive_remote(uint32_t cluster_addr) {
   asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
-// Descriptor of 32 rows of 16 bytes, one behind the other (no swizzle): 8-row groups are 128 bytes apart.
-__device__ __forceinline__ uint64_t smem_desc_rows16(uint32_t smem_addr) {
-  return (uint64_t)((smem_addr & 0x3FFFFu) >> 4) | (uint64_t)1 << 16 | (uint64_t)(128 >> 4) << 32 | (uint64_t)1 << 46;
-}
-// Instruction descriptor for kind::mxf4: A = B = E2M1, both K-major, E8M0 scales, K 64.
-__host__ __device__ constexpr uint32_t idesc_mxf4(int m, int n) {
-  return (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | (1u << 23) | ((uint32_t)(m >> 4) << 24);
-}
-
-struct FcParams {
-  void *out;  // [M, N]
-  const float *bias;
-  int32_t *status;
-  int M, N, k_steps;  // k_steps: MMAs to a row, 64 elements each
-  int relu, store_by_tma;
-};
-
 // Tensor memory (512 columns): two accumulators, then the scales of the k-blocks in flight.  Two accumulators of 256
 // columns would leave no room for the scales, so they share kShared columns there: the epilogue empties those first, and
 // the next tile's MMAs start as soon as it has.
@@ -102,33 +78,6 @@ __device__ __forceinline__ void tma_store_2d(const CUtensorMap *map, const void 
                ::"l"(map), "r"(c0), "r"(c1), "r"(smem_u32(src))
                : "memory");
 }
-
-// One lane of a warp that runs together.  The loops that issue TMA loads and MMAs are walked by whole warps and only the
-// instructions are this lane's: their operands then stay in uniform registers.  In a loop of one lane of a divergent
-// warp every tcgen05 instruction took 60 to 95 clocks to issue, 1100 to 1270 a k-block, whatever the MMAs' size.
-__device__ __forceinline__ bool elect_one() {
-  uint32_t one;
-  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
-  return one != 0;
-}
-
-// mbar_wait by a whole warp, whose lanes agree on the outcome.
-__device__ __forceinline__ bool warp_wait(uint64_t *bar, uint32_t parity, volatile int *abort_flag) {
-  return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag));
-}
-
-// Position in a ring of N places, and how often (even or odd) it has come round.
-template <int N>
-struct Ring {
-  int at = 0;
-  uint32_t round = 0;
-  __device__ __forceinline__ void next() {
-    if (++at == N) {
-      at = 0;
-      round ^= 1;
-    }
-  }
-};
 
 // Persistent: blocks, or pairs of them, walk the 128 x BLOCK_N (256 x BLOCK_N) tiles, row tile fastest (blocks that run
 // together share weights).  Warp 0 loads, warp 1 (of a pair's even block) issues the copies of the scales and the MMAs,
@@ -372,18 +321,6 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
   }
 }
 
-// [rows, pitch] bytes, box of 128 bytes by box_rows, 128-byte swizzle.
-int make_data_map(CUtensorMap *map, const void *base, int64_t rows, int64_t pitch, int box_rows) {
-  EncodeTiledFn fn = encode_tiled_fn();
-  if (!fn) return set_error(GLOWB200_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
-  cuuint64_t dims[2] = {(cuuint64_t)pitch, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)pitch};
-  cuuint32_t box[2] = {(cuuint32_t)kBlockK, (cuuint32_t)box_rows}, estr[2] = {1, 1};
-  CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void *>(base), dims, strides, box, estr,
-                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  if (r != CUDA_SUCCESS) return set_error(GLOWB200_ERR_CUDA, "cuTensorMapEncodeTiled failed with CUresult %d", (int)r);
-  return GLOWB200_OK;
-}
 // the result [M, N]: boxes of 32 rows by 128 bytes, in the 128-byte swizzle
 int make_out_map(CUtensorMap *map, const FcParams &p, int bytes) {
   EncodeTiledFn fn = encode_tiled_fn();
@@ -396,19 +333,6 @@ int make_out_map(CUtensorMap *map, const FcParams &p, int bytes) {
   if (r != CUDA_SUCCESS) return set_error(GLOWB200_ERR_CUDA, "cuTensorMapEncodeTiled failed with CUresult %d", (int)r);
   return GLOWB200_OK;
 }
-// scale tiles [row tiles, tiles * 512 bytes] as words: a box is two tiles (256 words) of box_tiles row tiles.
-int make_scale_map(CUtensorMap *map, const void *base, int64_t row_tiles, int64_t tiles, int box_tiles) {
-  EncodeTiledFn fn = encode_tiled_fn();
-  if (!fn) return set_error(GLOWB200_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
-  cuuint64_t dims[2] = {(cuuint64_t)tiles * 128, (cuuint64_t)row_tiles}, strides[1] = {(cuuint64_t)tiles * 512};
-  cuuint32_t box[2] = {256, (cuuint32_t)box_tiles}, estr[2] = {1, 1};
-  CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT32, 2, const_cast<void *>(base), dims, strides, box, estr,
-                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  if (r != CUDA_SUCCESS) return set_error(GLOWB200_ERR_CUDA, "cuTensorMapEncodeTiled failed with CUresult %d", (int)r);
-  return GLOWB200_OK;
-}
-
 template <int BLOCK_N, int STAGES, bool PAIR, typename Out>
 int launch_tiles(const void *a, const void *sa, const void *b, const void *sb, int64_t K, FcParams p, cudaStream_t s) {
   using S = Tile<BLOCK_N, STAGES, PAIR, Out>;
@@ -486,9 +410,15 @@ int check_fc(const void *out, int out_type, const void *in, const void *weights,
   return GLOWB200_OK;
 }
 
+FcParams fc_params(void *out, const float *bias, int64_t M, int64_t K, int64_t N, int flags, int32_t *status) {
+  return {out, bias, status, (int)M, (int)N, (int)((K + 63) / 64), (flags & GLOWB200_FC_FUSE_RELU) != 0, 0};
+}
+
 int run_fc(void *out, int out_type, const void *a, const void *sa, const void *b, const void *sb, const float *bias, int64_t M, int64_t K,
            int64_t N, int flags, int32_t *status, cudaStream_t s) {
-  const FcParams p{out, bias, status, (int)M, (int)N, (int)((K + 63) / 64), (flags & GLOWB200_FC_FUSE_RELU) != 0, 0};
+  if (M <= kFewRows)
+    return run_fp4_few_rows(fc_params(out, bias, M, K, N, flags, status), out_type, a, sa, -1, 0, b, sb, K, s);
+  const FcParams p = fc_params(out, bias, M, K, N, flags, status);
   return with_float_type(out_type, [&](auto *t) {
     return launch<std::remove_pointer_t<decltype(t)>>(a, sa, b, sb, K, p, s);
   });
@@ -527,6 +457,9 @@ extern "C" int glowb200_dynamic_microscaled_fp4_fc(void *out, int out_type, cons
   if (workspace == nullptr || workspace_bytes < need)
     return set_error(GLOWB200_ERR_WORKSPACE_TOO_SMALL, "workspace of %zu bytes given, %zu needed", workspace_bytes, need);
   GLOWB200_REQUIRE(aligned(workspace, 256), "workspace must be 256-byte aligned");
+  if (M <= kFewQuantizedRows)
+    return run_fp4_few_rows(fc_params(out, bias, M, K, N, flags, status), out_type, in, nullptr, in_type, row_stride, weights, weights_scales, K,
+                            reinterpret_cast<cudaStream_t>(stream));
   uint8_t *data = reinterpret_cast<uint8_t *>(workspace), *scales = data + align_up((size_t)(M * mx_pitch(K)), 256);
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   if (int rc = run_mx_quantize(in, in_type, M, K, row_stride, data, scales, s)) return rc;

@@ -29,29 +29,10 @@ __global__ void __launch_bounds__(kQuantThreads) mx_quantize_kernel(const T *__r
     const int64_t row = row_tile * 128 + r;
     if (row_tile * 128 + i * 16 + (first & ~1) >= rows) break;  // (of the warp's two rows the first: all lanes leave together)
     const bool real = row < rows;
-    float v[8];
-    const T *x = in + row * row_stride + col;
-    if (VEC && real && col + 8 <= cols) {
-      __align__(16) T w[8];
-#pragma unroll
-      for (int k = 0; k < (int)(8 * sizeof(T) / 16); k++)
-        reinterpret_cast<uint4 *>(w)[k] = reinterpret_cast<const uint4 *>(x)[k];
-#pragma unroll
-      for (int k = 0; k < 8; k++) v[k] = to_float(w[k]);
-    } else {
-#pragma unroll
-      for (int k = 0; k < 8; k++) v[k] = real && col + k < cols ? to_float(x[k]) : 0.0f;
-    }
-    uint32_t top = 0;
-#pragma unroll
-    for (int k = 0; k < 8; k++) top = max(top, __float_as_uint(v[k]) & 0x7FFFFFFFu);
-    top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-    top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-    const uint32_t byte = mx_scale_byte(top);
-    const float inverse = mx_inverse_scale(byte == 255u ? 127u : byte);
-#pragma unroll
-    for (int k = 0; k < 8; k++) v[k] *= inverse;
-    const uint32_t codes = byte == 255u ? 0u : mx_codes(v);
+    Eight<VEC, T> x;
+    x.load(in + row * row_stride + col, real ? cols - col : 0);
+    uint32_t byte;
+    const uint32_t codes = mx_block(x, byte);
     if (real && col / 2 < pitch) {  // (pitch: whole blocks)
       *reinterpret_cast<uint32_t *>(data + row * pitch + col / 2) = codes;
       if ((lane & 3) == 0) tile[(r & 31) * 16 + (r >> 5) * 4 + ((lane & 15) >> 2)] = (uint8_t)byte;

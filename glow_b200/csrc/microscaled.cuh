@@ -71,6 +71,38 @@ __device__ __forceinline__ uint32_t mx_codes(const float (&v)[8]) {
       : "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]));
   return r;
 }
+// Eight neighbours of a row from `x` on, `left` of which are there (the others are zeros).  VEC: x is on a 16-byte boundary.
+template <bool VEC, typename T>
+struct Eight {
+  __align__(16) T w[8];
+  __device__ __forceinline__ void load(const T *x, int64_t left) {
+    if (VEC && left >= 8) {
+#pragma unroll
+      for (int k = 0; k < (int)(8 * sizeof(T) / 16); k++) reinterpret_cast<uint4 *>(w)[k] = __ldg(reinterpret_cast<const uint4 *>(x) + k);
+    } else {
+#pragma unroll
+      for (int k = 0; k < 8; k++) w[k] = k < left ? x[k] : from_float<T>(0.0f);
+    }
+  }
+};
+// A block of 32 numbers, eight to each of four neighbouring lanes (all 32 lanes take part): the lane's codes and the block's
+// scale byte.  Infinities and NaNs: byte 255, codes 0.
+template <bool VEC, typename T>
+__device__ __forceinline__ uint32_t mx_block(const Eight<VEC, T> &x, uint32_t &byte) {
+  float v[8];
+#pragma unroll
+  for (int k = 0; k < 8; k++) v[k] = to_float(x.w[k]);
+  uint32_t top = 0;
+#pragma unroll
+  for (int k = 0; k < 8; k++) top = max(top, __float_as_uint(v[k]) & 0x7FFFFFFFu);
+  top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+  top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+  byte = mx_scale_byte(top);
+  const float inverse = mx_inverse_scale(byte == 255u ? 127u : byte);
+#pragma unroll
+  for (int k = 0; k < 8; k++) v[k] *= inverse;
+  return byte == 255u ? 0u : mx_codes(v);
+}
 // Two codes (a byte) -> their numbers.
 __device__ __forceinline__ float2 mx_numbers(uint32_t byte) {
   uint32_t h;
