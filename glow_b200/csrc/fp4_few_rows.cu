@@ -38,9 +38,6 @@ __device__ __forceinline__ float4 ld_cluster(uint32_t addr) {
   asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
   return v;
 }
-// Descriptors of tensor maps come from memory the first time; this needs no wait for the kernel before.
-__device__ __forceinline__ void prefetch_map(const CUtensorMap *map) { asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory"); }
-
 // In: void = packed input, loaded by TMA.
 template <int NT, typename In, bool VEC, typename Out>
 __global__ void __launch_bounds__(kThreads, FewRows<NT>::kAtOnce)
@@ -109,11 +106,13 @@ fp4_few_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
     }
   } else if (warp == 1) {
     Ring<S::kStages> ring;
-    bool live = true;
-    for (int kb = first; kb < last; kb++, ring.next()) {
+    bool ready = mbar_try_wait(&full[0], 0);
+    for (int kb = first; kb < last; kb++) {
       const int s = ring.at;
-      if (!warp_wait(&full[s], ring.round, abort_flag)) { live = false; break; }
+      if (!__all_sync(0xffffffffu, ready) && !warp_wait(&full[s], ring.round, abort_flag)) break;
       tc_fence_after();
+      ring.next();
+      ready = kb + 1 < last && mbar_try_wait(&full[ring.at], ring.round);
       const uint32_t a_addr = smem_u32(smem + s * (S::kABytes + S::kBBytes)), sa_addr = smem_u32(scales + s * 2048);
       const uint64_t a_desc = smem_desc_sw128(a_addr), b_desc = smem_desc_sw128(a_addr + S::kABytes);
       const uint32_t t_sa = tmem_base + NT + (uint32_t)s * S::kScaleCols, t_sb = t_sa + 8;
@@ -131,12 +130,11 @@ fp4_few_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
             umma_mxf4<false>(tmem_base, a_desc + (uint64_t)(k * (kUmmaK >> 4)), b_desc + (uint64_t)(k * (kUmmaK >> 4)),
                              idesc_mxf4(kBlockM, NT) | id << 4 | id << 29, t_sa + 4 * (k >> 1), t_sb + 4 * (k >> 1), kb != first || k != 0);
         }
-        umma_commit(&empty[s]);
+        if (kb + S::kStages < last) umma_commit(&empty[s]);  // (nobody waits for a stage that is not filled again)
         if (kb + 1 == last) umma_commit(acc_full);
       }
       __syncwarp();
     }
-    (void)live;
   } else {
     const int w = warp - 2;
     if constexpr (!kPacked) {

@@ -113,6 +113,13 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
+  if (threadIdx.x == 64) {
+    prefetch_map(&map_a);
+    prefetch_map(&map_sa);
+    prefetch_map(&map_b);
+    prefetch_map(&map_sb);
+    prefetch_map(&map_out);
+  }
   if (warp == 1) {
     if constexpr (PAIR) {
       tmem_alloc_pair(tmem_slot, 512);
@@ -416,7 +423,11 @@ FcParams fc_params(void *out, const float *bias, int64_t M, int64_t K, int64_t N
 
 int run_fc(void *out, int out_type, const void *a, const void *sa, const void *b, const void *sb, const float *bias, int64_t M, int64_t K,
            int64_t N, int flags, int32_t *status, cudaStream_t s) {
-  if (M <= kFewRows)
+  // The other kernel's time grows with the rows, which it adds up over a cluster, and shrinks with its splits of the depth: 64 rows
+  // of 4096 x 4096 (K 1024, N 1024) 7.3 us (4.7) there and 7.1 (3.7) here, 32 rows 6.0 (4.1), 16 rows 5.2 (3.7), 64 rows of K
+  // 16384, N 2048 8.7 and 18.4, 128 rows of it 16.4.
+  const int64_t k_blocks = (K + 255) / 256;
+  if (M <= 16 || (M <= 64 && k_blocks >= 8) || (M <= kFewRows && k_blocks >= 32))
     return run_fp4_few_rows(fc_params(out, bias, M, K, N, flags, status), out_type, a, sa, -1, 0, b, sb, K, s);
   const FcParams p = fc_params(out, bias, M, K, N, flags, status);
   return with_float_type(out_type, [&](auto *t) {

@@ -74,6 +74,9 @@ __device__ __forceinline__ bool elect_one() {
   return one != 0;
 }
 
+// Descriptors of tensor maps come from memory the first time; this needs no wait for the kernel before.
+__device__ __forceinline__ void prefetch_map(const CUtensorMap *map) { asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory"); }
+
 // mbar_wait by a whole warp, whose lanes agree on the outcome.
 __device__ __forceinline__ bool warp_wait(uint64_t *bar, uint32_t parity, volatile int *abort_flag) {
   return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag));
