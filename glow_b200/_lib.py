@@ -99,7 +99,7 @@ SIGNATURES = {
         _int, [_vp, _int, _vp, _int, _i64, _vp, _vp, _vp, _i64, _i64, _i64, _int, _vp, _sz, _vp, _vp]),
     "glowb200_group_norm_workspace_bytes": (_sz, [_i64] * 4),
     "glowb200_group_norm": (
-        _int, [_vp, _int, _vp, _f32, _i32, _vp, _int, _vp, _vp] + [_i64] * 4 + [_f32, _int, _vp, _sz, _vp]),
+        _int, [_vp, _int, _vp, _f32, _i32, _vp, _int, _vp, _vp] + [_i64] * 4 + [_f32, _int, _vp, _sz, _vp, _vp]),
     "glowb200_peer_buffer_create": (_int, [_sz, _vp, _vp]),
     "glowb200_peer_buffer_open": (_int, [_vp, _vp]),
     "glowb200_peer_buffer_close": (_int, [_vp]),

@@ -695,7 +695,7 @@ PyObject *mx_dynamic_fc(PyObject *const *a) {
   return a[6] == Py_None ? give(out) : same(a[6]);
 }
 
-// x, groups, gamma, beta, eps, activation, quantized?, scale, offset, out type, out, workspace
+// x, groups, gamma, beta, eps, activation, quantized?, scale, offset, out type, out, workspace, status
 PyObject *group_norm(PyObject *const *a) {
   const Tensor &x = cuda_tensor(a[0], "x", FLOATS);
   if (x.dim() < 2) bad_value("%s must have images first and channels last", "x");
@@ -712,7 +712,7 @@ PyObject *group_norm(PyObject *const *a) {
   beside(room.t, "workspace", x);
   invoke(fn.glowb200_group_norm, quant ? nullptr : out.data_ptr(), quant ? 0 : float_type(type), quant ? (int8_t *)out.data_ptr() : nullptr,
          real(a[7]), (int32_t)integer(a[8]), x.data_ptr(), float_type(x.scalar_type()), gamma, beta, images, pixels, channels, groups,
-         real(a[4]), (int)integer(a[5]), room.data(), room.bytes(), stream());
+         real(a[4]), (int)integer(a[5]), room.data(), room.bytes(), status_word(a[12], x), stream());
   return a[10] == Py_None ? give(out) : same(a[10]);
 }
 
@@ -822,7 +822,7 @@ PyMethodDef methods[] = {
     FAST("mx_dequantize", mx_dequantize, 5),
     FAST("mx_fc", mx_fc, 9),
     FAST("mx_dynamic_fc", mx_dynamic_fc, 9),
-    FAST("group_norm", group_norm, 12),
+    FAST("group_norm", group_norm, 13),
     FAST("run_function", run_function, 4),
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_binding", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

@@ -63,16 +63,6 @@ struct Tile {
   static_assert(kScalesAt + STAGES * kScaleCols <= 512 && kShared % kChunk == 0, "tensor memory");
 };
 
-__device__ __forceinline__ uint32_t pack2(float lo, float hi, __half) {
-  uint32_t r;
-  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-  return r;
-}
-__device__ __forceinline__ uint32_t pack2(float lo, float hi, __nv_bfloat16) {
-  uint32_t r;
-  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-  return r;
-}
 __device__ __forceinline__ void tma_store_2d(const CUtensorMap *map, const void *src, int c0, int c1) {
   asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];"
                ::"l"(map), "r"(c0), "r"(c1), "r"(smem_u32(src))

@@ -15,6 +15,7 @@
 #include <cstdlib>
 
 #include "microscaled.cuh"
+#include "tcgen05.cuh"
 
 namespace glowb200 {
 namespace {
@@ -28,6 +29,7 @@ struct NormParams {
   const float *gamma, *beta;
   float2 *partial;  // [images][groups][chunks] mean, M2
   float2 *stats;    // [images][groups] mean, 1 / sqrt(var + eps)
+  int32_t *status;
   int64_t images, pixels;
   int channels, groups, chunks;
   int64_t chunk_pixels;
@@ -37,226 +39,422 @@ struct NormParams {
   int act;
 };
 
+// Two floats in a register pair, for the two-lane instructions.
+struct Two {
+  uint64_t v;
+  __device__ __forceinline__ Two() {}
+  __device__ __forceinline__ Two(float a, float b) { asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b)); }
+  __device__ __forceinline__ float2 both() const {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+  }
+};
+__device__ __forceinline__ Two operator+(Two a, Two b) {
+  Two r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ Two operator*(Two a, Two b) {
+  Two r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ Two fma2(Two a, Two b, Two c) {
+  Two r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+// Two 16-bit numbers of a word, widened: fp16 through the mixed-precision add (conversions issue at an eighth of its rate),
+// bf16 by its place.
+__device__ __forceinline__ Two widen(uint32_t w, __half) {
+  float a, b;
+  asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tadd.rn.f32.f16 %0, l, %3;\n\tadd.rn.f32.f16 %1, h, %3;\n\t}" : "=f"(a), "=f"(b) : "r"(w), "f"(-0.0f));
+  return Two(a, b);
+}
+__device__ __forceinline__ Two widen(uint32_t w, __nv_bfloat16) { return Two(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u)); }
+
+template <int N>
+struct Known {  // a number known when compiled, and one that is not (value 0)
+  static constexpr int value = N;
+  __device__ __forceinline__ constexpr operator int() const { return N; }
+};
+struct Count {
+  static constexpr int value = 0;
+  int n;
+  __device__ __forceinline__ operator int() const { return n; }
+};
 __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
   return v;
 }
-// A warp joins parts of one group, of which at(i) gives mean, M2 and, by `n`, the number: all lanes get mean and M2 of the
-// whole.  (The mean first, then what the parts' own means differ from it: no quotient but the one.)
-template <typename At>
+// A warp joins parts of one group, of which at(i, n) gives mean and M2 and sets the number: all lanes get mean and M2 of the
+// whole.  (The mean first, then what the parts' own means differ from it: no quotient but the one.)  MOST: parts of a
+// lane that are asked for before the first is used; more come twice.
+template <int MOST, typename At>
 __device__ __forceinline__ float2 join_parts(int count, float total, At at) {
   const int lane = threadIdx.x & 31;
-  float sum = 0.0f, squares = 0.0f, n;
-  for (int i = lane; i < count; i += 32) {
-    const float2 v = at(i, n);
-    sum = fmaf(n, v.x, sum);
-    squares += v.y;
+  float sum = 0.0f, squares = 0.0f, n[MOST];
+  float2 v[MOST];
+#pragma unroll
+  for (int k = 0; k < MOST; k++) {
+    n[k] = 0.0f;
+    v[k] = make_float2(0.0f, 0.0f);
+    if (lane + 32 * k < count) v[k] = at(lane + 32 * k, n[k]);
+  }
+#pragma unroll
+  for (int k = 0; k < MOST; k++) {
+    sum = fmaf(n[k], v[k].x, sum);
+    squares += v[k].y;
+  }
+  for (int i = lane + 32 * MOST; i < count; i += 32) {
+    float m;
+    const float2 w = at(i, m);
+    sum = fmaf(m, w.x, sum);
+    squares += w.y;
   }
   const float mean = warp_sum(sum) / total;
-  for (int i = lane; i < count; i += 32) {
-    const float2 v = at(i, n);
-    const float d = v.x - mean;
-    squares = fmaf(n * d, d, squares);
+#pragma unroll
+  for (int k = 0; k < MOST; k++) {
+    const float d = v[k].x - mean;
+    if (n[k] > 0.0f) squares = fmaf(n[k] * d, d, squares);
+  }
+  for (int i = lane + 32 * MOST; i < count; i += 32) {
+    float m;
+    const float2 w = at(i, m);
+    const float d = w.x - mean;
+    squares = fmaf(m * d, d, squares);
   }
   return make_float2(mean, warp_sum(squares));
 }
 
+// VEC neighbours, as they are loaded and stored: words, or one element.
 template <typename T, int VEC>
-struct alignas(sizeof(T) * VEC) Pack {
-  T v[VEC];
+struct Pack {
+  static constexpr int kWords = sizeof(T) * VEC / 4 > 0 ? sizeof(T) * VEC / 4 : 1, kTwos = (VEC + 1) / 2;
+  uint32_t w[kWords];
+  __device__ __forceinline__ void load(const T *p) {
+    if constexpr (kWords == 4) {
+      const uint4 r = *reinterpret_cast<const uint4 *>(p);
+      w[0] = r.x, w[1] = r.y, w[2] = r.z, w[3] = r.w;
+    } else if constexpr (sizeof(T) * VEC == 4) {
+      w[0] = *reinterpret_cast<const uint32_t *>(p);
+    } else {
+      w[0] = *reinterpret_cast<const uint16_t *>(p);
+    }
+  }
+  __device__ __forceinline__ Two two(int i) const {  // elements 2i and 2i + 1 (of one element: it and 0)
+    if constexpr (sizeof(T) == 4) return Two(__uint_as_float(w[VEC > 1 ? 2 * i : 0]), VEC > 1 ? __uint_as_float(w[2 * i + (VEC > 1)]) : 0.0f);
+    else return widen(w[i], T());
+  }
 };
-template <typename P>
-__device__ __forceinline__ P load_pack(const P *p) {
-  P r;
-  if constexpr (sizeof(P) == 16) *reinterpret_cast<uint4 *>(&r) = *reinterpret_cast<const uint4 *>(p);
-  else if constexpr (sizeof(P) == 8) *reinterpret_cast<uint2 *>(&r) = *reinterpret_cast<const uint2 *>(p);
-  else if constexpr (sizeof(P) == 4) *reinterpret_cast<uint32_t *>(&r) = *reinterpret_cast<const uint32_t *>(p);
-  else r = *p;
-  return r;
-}
-// (read for the last time)
-template <typename P>
-__device__ __forceinline__ P load_last(const P *p) {
-  P r;
-  if constexpr (sizeof(P) == 16) *reinterpret_cast<uint4 *>(&r) = __ldcs(reinterpret_cast<const uint4 *>(p));
-  else if constexpr (sizeof(P) == 4) *reinterpret_cast<uint32_t *>(&r) = __ldcs(reinterpret_cast<const uint32_t *>(p));
-  else r = load_pack(p);
-  return r;
-}
-// (not read again here)
-template <typename P>
-__device__ __forceinline__ void store_pack(P *p, const P &r) {
-  if constexpr (sizeof(P) == 32) {
-    __stcs(reinterpret_cast<uint4 *>(p), reinterpret_cast<const uint4 *>(&r)[0]);
-    __stcs(reinterpret_cast<uint4 *>(p) + 1, reinterpret_cast<const uint4 *>(&r)[1]);
-  } else if constexpr (sizeof(P) == 16) {
-    __stcs(reinterpret_cast<uint4 *>(p), *reinterpret_cast<const uint4 *>(&r));
-  } else if constexpr (sizeof(P) == 8) {
-    __stcs(reinterpret_cast<uint2 *>(p), *reinterpret_cast<const uint2 *>(&r));
-  } else if constexpr (sizeof(P) == 4) {
-    __stcs(reinterpret_cast<uint32_t *>(p), *reinterpret_cast<const uint32_t *>(&r));
-  } else {
-    *p = r;
+// What follows the normalisation of some numbers.
+template <typename Out, int N>
+__device__ __forceinline__ void activate(float (&y)[N], int act) {
+  if (act == GLOWB200_NORM_ACT_RELU) {
+#pragma unroll
+    for (int k = 0; k < N; k++) asm("max.NaN.f32 %0, %0, %1;" : "+f"(y[k]) : "f"(0.0f));
+  } else if (act == GLOWB200_NORM_ACT_SWISH) {
+    // (16-bit results: the fast exponential and quotient are off by some 2^-21)
+#pragma unroll
+    for (int k = 0; k < N; k++) {
+      if constexpr (sizeof(Out) == 2) y[k] = __fdividef(y[k], 1.0f + __expf(-y[k]));
+      else y[k] = y[k] / (1.0f + expf(-y[k]));
+    }
   }
 }
 
-// Statistics of `groups` groups of `width` channels over `pixels` pixels: x is the first of them, in pixels of `channels`
-// channels.  Thread t of the first columns * rows has VEC channels (column t % columns) of every rows-th pixel; UNIT: how
-// many neighbours of them lie in one group.  Lane 0 of the warp that gets a group calls done(group, {mean, M2}).
-template <typename T, int VEC, int UNIT, typename Done>
-__device__ __forceinline__ void group_parts(const T *x, int pixels, int channels, int groups, int width, int rows, float2 *shared, Done done) {
-  constexpr int kBatch = VEC >= 8 ? 4 : 8, kUnits = VEC / UNIT;
-  const int columns = groups * width / VEC, t = threadIdx.x, row = t / columns, column = t - row * columns;
-  const int base = pixels / rows, extra = pixels - base * rows;  // row r has base pixels, the first `extra` rows one more
-  if (row < rows) {
-    float mean[VEC], squares[VEC], n = 0.0f;
+// max(x, 0) of two 16-bit numbers, NaN staying NaN
+__device__ __forceinline__ uint32_t relu2(uint32_t w, __half) {
+  asm("max.NaN.f16x2 %0, %0, %1;" : "+r"(w) : "r"(0u));
+  return w;
+}
+__device__ __forceinline__ uint32_t relu2(uint32_t w, __nv_bfloat16) {
+  asm("max.NaN.bf16x2 %0, %0, %1;" : "+r"(w) : "r"(0u));
+  return w;
+}
+// (results: not read again here)
+template <typename Out, int VEC>
+__device__ __forceinline__ void store_results(Out *p, float (&y)[VEC], const NormParams &q, int act) {
+  constexpr bool kPairs = sizeof(Out) == 2 && VEC > 1;  // Relu after the rounding, two at a time
+  if (act == GLOWB200_NORM_ACT_SWISH || (!kPairs && act == GLOWB200_NORM_ACT_RELU)) activate<Out>(y, act);
+  if constexpr (sizeof(Out) == 1) {  // quantization::quantize<int8_t>, as the Quantize node
+    uint32_t w[(VEC + 3) / 4] = {};
 #pragma unroll
-    for (int k = 0; k < VEC; k++) mean[k] = squares[k] = 0.0f;
-    const T *at = x + (int64_t)row * channels + column * VEC;
-    const int64_t step = (int64_t)rows * channels;
-    int left = base + (row < extra ? 1 : 0);
-    auto take = [&](const Pack<T, VEC> *p, auto count_tag) {
-      constexpr int kCount = decltype(count_tag)::value;
-      const float share = __fdividef((float)kCount, n + (float)kCount), cross = n * share;
+    for (int k = 0; k < VEC; k++) {
+      const long long v = (long long)rintf(__fadd_rn(__fdiv_rn(y[k], q.quant_scale), (float)q.quant_offset));
+      w[k / 4] |= (uint32_t)(uint8_t)(v < -128 ? -128 : (v > 127 ? 127 : v)) << (8 * (k % 4));
+    }
+    if constexpr (VEC == 8) *reinterpret_cast<uint2 *>(p) = make_uint2(w[0], w[1]);
+    else if constexpr (VEC == 4) *reinterpret_cast<uint32_t *>(p) = w[0];
+    else if constexpr (VEC == 2) *reinterpret_cast<uint16_t *>(p) = (uint16_t)w[0];
+    else *reinterpret_cast<uint8_t *>(p) = (uint8_t)w[0];
+  } else if constexpr (VEC == 1) {
+    *p = from_float<Out>(y[0]);
+  } else if constexpr (sizeof(Out) == 2) {
+    uint32_t w[VEC / 2];
 #pragma unroll
-      for (int k = 0; k < VEC; k++) {
-        float v[kCount], m = 0.0f, q = 0.0f;
+    for (int k = 0; k < VEC / 2; k++) w[k] = pack2(y[2 * k], y[2 * k + 1], Out());
+    if (act == GLOWB200_NORM_ACT_RELU) {
 #pragma unroll
-        for (int i = 0; i < kCount; i++) {
-          v[i] = to_float(p[i].v[k]);
-          m += v[i];
-        }
-        m *= 1.0f / (float)kCount;
+      for (int k = 0; k < VEC / 2; k++) w[k] = relu2(w[k], Out());
+    }
+    if constexpr (VEC == 8) __stcs(reinterpret_cast<uint4 *>(p), make_uint4(w[0], w[1], w[2], w[3]));
+    else if constexpr (VEC == 4) __stcs(reinterpret_cast<uint2 *>(p), make_uint2(w[0], w[1]));
+    else *reinterpret_cast<uint32_t *>(p) = w[0];
+  } else if constexpr (VEC == 2) {
+    *reinterpret_cast<float2 *>(p) = make_float2(y[0], y[1]);
+  } else {
 #pragma unroll
-        for (int i = 0; i < kCount; i++) {
-          const float d = v[i] - m;
-          q = fmaf(d, d, q);
-        }
-        const float d = m - mean[k];
-        mean[k] = fmaf(d, share, mean[k]);
-        squares[k] += fmaf(d * d, cross, q);
-      }
-      n += (float)kCount;
-    };
-    for (; left >= kBatch; left -= kBatch) {
-      Pack<T, VEC> p[kBatch];
+    for (int k = 0; k < VEC; k += 4) __stcs(reinterpret_cast<float4 *>(p + k), make_float4(y[k], y[k + 1], y[k + 2], y[k + 3]));
+  }
+}
+
+// A block's pixels by plain loads: calls body(pixels, how many, the first one's place) for those of this thread, `left` from
+// `at` on.
+template <typename T, int VEC>
+struct Loads {
+  static constexpr int kBatch = 4;
+  const T *at;
+  int64_t step;
+  int left;
+  template <typename Body>
+  __device__ __forceinline__ void each(Body body) {
+    Pack<T, VEC> p[kBatch];
+    for (int first = 0; first < left; first += kBatch) {
 #pragma unroll
-      for (int i = 0; i < kBatch; i++) p[i] = load_pack(reinterpret_cast<const Pack<T, VEC> *>(at + i * step));
+      for (int i = 0; i < kBatch; i++)
+        if (first + i < left) p[i].load(at + i * step);
       at += kBatch * step;
-      take(p, std::integral_constant<int, kBatch>());
+      body(p, min(left - first, kBatch), first);
     }
-    {
-      Pack<T, VEC> p[kBatch - 1];
-#pragma unroll
-      for (int i = 0; i < kBatch - 1; i++)
-        if (i < left) p[i] = load_pack(reinterpret_cast<const Pack<T, VEC> *>(at + i * step));
-#pragma unroll
-      for (int i = 0; i < kBatch - 1; i++)
-        if (i < left) take(p + i, std::integral_constant<int, 1>());
-    }
-    // the channels of a unit, n numbers each: M2 = sum of theirs + n * (sum of squared differences of their means)
-#pragma unroll
-    for (int u = 0; u < kUnits; u++) {
-      float m = 0.0f, q = 0.0f, sum = 0.0f;
-#pragma unroll
-      for (int k = 0; k < UNIT; k++) m += mean[u * UNIT + k];
-      m *= 1.0f / (float)UNIT;
-#pragma unroll
-      for (int k = 0; k < UNIT; k++) {
-        const float d = mean[u * UNIT + k] - m;
-        sum += squares[u * UNIT + k];
-        q = fmaf(d, d, q);
+  }
+};
+
+// The same for whole pixels, which lie one behind the other: bulk copies bring eight of every thread at a time into a ring
+// in shared memory, ahead of the arithmetic.  Pieces of 16 bytes only.  What bounds these kernels beside the bytes is issue
+// slots: few warps with eight pixels at a time pay less of them for waiting and joining than many with four.
+constexpr int kStages = 3;
+template <typename T, int VEC>
+struct Stream {
+  static constexpr bool kCan = VEC * sizeof(T) == 16;
+  static constexpr int kBatch = 8;
+  __host__ __device__ static constexpr int bytes(int threads) { return kCan ? kStages * threads * 16 * kBatch + 128 : 0; }
+  const uint8_t *x;
+  uint8_t *ring;
+  uint64_t *full, *empty;
+  volatile int *gave_up;
+  int pixels, rows, stages, stage_bytes;
+  uint32_t pixel_bytes;
+  bool backwards;  // from the last stage to the first
+
+  __device__ __forceinline__ int stage_of(int j) const { return backwards ? stages - 1 - j : j; }
+  __device__ __forceinline__ void ask(int j) const {  // (by one thread)
+    const int first = stage_of(j) * kBatch * rows, slot = j % kStages;
+    const uint32_t size = (uint32_t)min(kBatch * rows, pixels - first) * pixel_bytes;
+    mbar_expect_tx(&full[slot], size);
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                 ::"r"(smem_u32(ring + slot * stage_bytes)), "l"(x + (int64_t)first * pixel_bytes), "r"(size), "r"(smem_u32(&full[slot]))
+                 : "memory");
+  }
+  // By all threads: barriers, and the first stages on their way.
+  __device__ __forceinline__ Stream(const T *from, int pixels, int channels, int rows, void *shared, bool backwards)
+      : x(reinterpret_cast<const uint8_t *>(from)), ring(reinterpret_cast<uint8_t *>(shared)), pixels(pixels), rows(rows),
+        stages((pixels + kBatch * rows - 1) / (kBatch * rows)), stage_bytes(blockDim.x * 16 * kBatch),
+        pixel_bytes(channels * (uint32_t)sizeof(T)), backwards(backwards) {
+    full = reinterpret_cast<uint64_t *>(ring + kStages * stage_bytes);
+    empty = full + kStages;
+    gave_up = reinterpret_cast<volatile int *>(empty + kStages);
+    if (threadIdx.x == 0) {
+      for (int s = 0; s < kStages; s++) {
+        mbar_init(&full[s], 1);
+        mbar_init(&empty[s], blockDim.x >> 5);
       }
-      shared[t * kUnits + u] = make_float2(m, fmaf(n, q, sum));
+      *gave_up = 0;
+      asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+      for (int j = 0; j < kStages && j < stages; j++) ask(j);
+    }
+    __syncthreads();
+  }
+  // body(pixels, how many, the first one's place among this thread's)
+  template <typename Body>
+  __device__ __forceinline__ void each(Body body) {
+    const int t = threadIdx.x, columns = (int)(pixel_bytes >> 4), row = t / columns;
+    const int mine = row < rows && row < pixels ? (pixels - row + rows - 1) / rows : 0;  // pixels of this thread
+    const uint32_t place = smem_u32(ring) + 16 * t, apart = 16 * rows * columns;
+    int slot = 0;
+    uint32_t round = 0;
+    for (int j = 0; j < stages; j++) {
+      if (!__all_sync(0xffffffffu, mbar_wait(&full[slot], round, gave_up))) return;
+      const int first = stage_of(j) * kBatch, count = min(kBatch, mine - first);
+      Pack<T, VEC> p[kBatch];
+      auto read = [&](int i) {
+        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                     : "=r"(p[i].w[0]), "=r"(p[i].w[1]), "=r"(p[i].w[2]), "=r"(p[i].w[3])
+                     : "r"(place + slot * stage_bytes + i * apart)
+                     : "memory");
+      };
+      if (count == kBatch) {
+#pragma unroll
+        for (int i = 0; i < kBatch; i++) read(i);
+      } else {
+#pragma unroll
+        for (int i = 0; i < kBatch; i++)
+          if (i < count) read(i);
+      }
+      __syncwarp();
+      if ((t & 31) == 0) mbar_arrive(&empty[slot]);
+      // the stage before this one is filled again once every warp has read it
+      if (t < 32 && j > 0 && j - 1 + kStages < stages) {
+        const int before = slot == 0 ? kStages - 1 : slot - 1;
+        if (!__all_sync(0xffffffffu, mbar_wait(&empty[before], slot == 0 ? round ^ 1 : round, gave_up))) return;
+        if (t == 0) ask(j - 1 + kStages);
+        __syncwarp();
+      }
+      if (count > 0) body(p, count, first);
+      if (++slot == kStages) {
+        slot = 0;
+        round ^= 1;
+      }
+    }
+  }
+  // By all threads, at the end: a wait that gave up is reported, copies on their way get a bounded time to land.
+  __device__ __forceinline__ void finish(int32_t *status) const {
+    __syncthreads();
+    if (*gave_up) {
+      if (threadIdx.x == 0 && status != nullptr) atomicOr(status, GLOWB200_STATUS_WAIT_TIMEOUT);
+      const long long t0 = clock64();
+      while (clock64() - t0 < 4000000ll) {
+      }
+      __syncthreads();
+    }
+  }
+};
+
+// Statistics of `groups` groups of `width` channels over `pixels` pixels, which `source` hands out.  Thread t of the first columns * rows has VEC channels (column t % columns) of every
+// rows-th pixel; UNIT: how many neighbours of them lie in one group.  Lane 0 of the warp that gets a group calls done(group, {mean, M2}).
+template <typename T, int VEC, int UNIT, typename Source, typename Done>
+__device__ __forceinline__ void group_parts(Source source, int pixels, int groups, int width, int rows, float2 *shared, Done done) {
+  // A unit's numbers are one sum; units of one channel come two to a register pair.
+  constexpr int kBatch = Source::kBatch, kUnits = VEC / UNIT, kTwos = Pack<T, VEC>::kTwos, kSums = UNIT > 1 ? kUnits : kTwos, kEach = UNIT > 1 ? UNIT / 2 : 1;
+  const int columns = groups * width / VEC, t = threadIdx.x, row = t / columns;
+  const int base = pixels / rows, extra = pixels - base * rows;  // row r has base pixels, the first `extra` rows one more
+  {
+    Two mean[kSums], squares[kSums];  // (UNIT > 1: both halves of a mean are the same, those of M2 are to be added)
+    float n = 0.0f;
+#pragma unroll
+    for (int k = 0; k < kSums; k++) mean[k] = squares[k] = Two(0.0f, 0.0f);
+    // `count` of kBatch pixels: their mean, the squares of what they differ from it, and those joined to what was before.
+    auto take = [&](const auto &p, auto count) {
+      const float many = (float)count, numbers = many * (float)UNIT;
+      const float each = decltype(count)::value ? 1.0f / (float)(decltype(count)::value * UNIT) : __fdividef(1.0f, numbers);
+      const float share = __fdividef(many, n + many), cross = (UNIT > 1 ? 0.5f : 1.0f) * n * share * (float)UNIT;
+      const Two minus_share(-share, -share), crosses(cross, cross);
+#pragma unroll
+      for (int u = 0; u < kSums; u++) {
+        Two x[kBatch][kEach], sum, q;
+#pragma unroll
+        for (int i = 0; i < kBatch; i++)
+          if (i < count) {
+#pragma unroll
+            for (int k = 0; k < kEach; k++) {
+              x[i][k] = p[i].two(u * kEach + k);
+              sum = i == 0 && k == 0 ? x[i][k] : sum + x[i][k];
+            }
+          }
+        const float2 halves = sum.both();
+        const Two less = UNIT > 1 ? Two(-each * (halves.x + halves.y), -each * (halves.x + halves.y)) : Two(-each * halves.x, -each * halves.y);
+#pragma unroll
+        for (int i = 0; i < kBatch; i++)
+          if (i < count) {
+#pragma unroll
+            for (int k = 0; k < kEach; k++) {
+              const Two d = x[i][k] + less;
+              q = i == 0 && k == 0 ? d * d : fma2(d, d, q);
+            }
+          }
+        const Two d = mean[u] + less;
+        mean[u] = fma2(d, minus_share, mean[u]);
+        squares[u] = squares[u] + fma2(d * d, crosses, q);
+      }
+      n += many;
+    };
+    source.each([&](const auto &p, int count, int) {
+      if (count == kBatch) take(p, Known<kBatch>());
+      else take(p, Count{count});
+    });
+    if (row < rows)
+#pragma unroll
+    for (int u = 0; u < kSums; u++) {
+      const float2 m = mean[u].both(), q = squares[u].both();
+      if constexpr (UNIT > 1) {
+        shared[t * kUnits + u] = make_float2(m.x, q.x + q.y);
+      } else {
+        shared[t * kUnits + 2 * u] = make_float2(m.x, q.x);
+        if (VEC > 1) shared[t * kUnits + 2 * u + (VEC > 1)] = make_float2(m.y, q.y);
+      }
     }
   }
   __syncthreads();
   const int per_row = columns * kUnits, of_group = width / UNIT, warps = blockDim.x >> 5, lane = t & 31;
-  // units of a group, row by row: a lane walks them 32 at a time
-  const int first_row = lane / of_group, first_unit = lane - first_row * of_group, more_rows = 32 / of_group, more_units = 32 - more_rows * of_group;
+  const uint32_t reciprocal = 0xffffffffu / (uint32_t)of_group;
   const float few = (float)base * (float)UNIT, many = (float)(base + 1) * (float)UNIT, total = (float)pixels * (float)width;
   for (int g = t >> 5; g < groups; g += warps) {
-    int r = 0, u = 0;
-    const float2 part = join_parts(rows * of_group, total, [&](int i, float &n) {
-      if (i == lane) {
-        r = first_row;
-        u = first_unit;
-      } else {
-        r += more_rows;
-        u += more_units;
-        if (u >= of_group) {
-          u -= of_group;
-          r++;
-        }
-      }
+    const float2 part = join_parts<4>(rows * of_group, total, [&](int i, float &n) {  // units of the group, row by row
+      const int r = fast_div(i, of_group, reciprocal);
       n = r < extra ? many : few;
-      return shared[r * per_row + g * of_group + u];
+      return shared[r * per_row + g * of_group + (i - r * of_group)];
     });
     if (lane == 0) done(g, part);
   }
 }
 
-template <typename Out>
-__device__ __forceinline__ Out norm_result(float y, const NormParams &p) {
-  if (p.act == GLOWB200_NORM_ACT_RELU) {
-    y = y < 0.0f ? 0.0f : y;
-  } else if (p.act == GLOWB200_NORM_ACT_SWISH) {
-    // (16-bit results: the fast exponential and quotient are off by some 2^-21)
-    if constexpr (sizeof(Out) == 2) y = __fdividef(y, 1.0f + __expf(-y));
-    else y = y / (1.0f + expf(-y));
-  }
-  if constexpr (sizeof(Out) == 1) {  // quantization::quantize<int8_t>, as the Quantize node
-    const long long v = (long long)rintf(__fadd_rn(__fdiv_rn(y, p.quant_scale), (float)p.quant_offset));
-    return (int8_t)(v < -128 ? -128 : (v > 127 ? 127 : v));
-  } else {
-    return from_float<Out>(y);
-  }
-}
-
 // Normalises the same pixels; stats: mean and 1 / sqrt(var + eps) of the groups; c0: their first channel.
-template <typename T, int VEC, int UNIT, typename Out>
-__device__ __forceinline__ void normalise(const NormParams &p, const T *x, Out *y, int pixels, int groups, int width, int c0,
-                                          const float2 *stats) {
-  constexpr int kBatch = VEC >= 8 ? 4 : 8;
+template <typename T, int VEC, int UNIT, typename Out, typename Source>
+__device__ __forceinline__ void normalise(const NormParams &p, Source source, Out *y, int groups, int width, int c0, const float2 *stats) {
+  constexpr int kTwos = Pack<T, VEC>::kTwos;
   const int columns = groups * width / VEC, t = threadIdx.x, row = t / columns, column = t - row * columns;
-  if (row >= p.rows) return;
-  float mean[VEC], gain[VEC], shift[VEC];
+  // (x - mean) * gain + shift, the difference first: where a group's numbers hardly differ, gains are large
+  constexpr int kMeans = UNIT > 1 ? VEC / UNIT : kTwos, kEach = UNIT > 1 ? UNIT / 2 : 1;  // of register pairs
+  float less[VEC / UNIT + 1] = {}, gain[2 * kTwos] = {}, shift[2 * kTwos] = {};
+  if (row < p.rows)
 #pragma unroll
   for (int u = 0; u < VEC; u += UNIT) {
     const float2 s = stats[(column * VEC + u) / width];
+    less[u / UNIT] = -s.x;
 #pragma unroll
     for (int k = u; k < u + UNIT; k++) {
       const int c = c0 + column * VEC + k;
-      mean[k] = s.x;
       gain[k] = s.y * (p.gamma ? __ldg(p.gamma + c) : 1.0f);
       shift[k] = p.beta ? __ldg(p.beta + c) : 0.0f;
     }
   }
-  int64_t at = (int64_t)row * p.channels + column * VEC;
-  int left = row < pixels ? (pixels - row + p.rows - 1) / p.rows : 0;
-  const int64_t step = (int64_t)p.rows * p.channels;
-  auto one = [&](const Pack<T, VEC> &in, int64_t to) {
-    Pack<Out, VEC> out;
+  Two lesses[kMeans], gains[kTwos], shifts[kTwos];
 #pragma unroll
-    for (int k = 0; k < VEC; k++) out.v[k] = norm_result<Out>(fmaf(to_float(in.v[k]) - mean[k], gain[k], shift[k]), p);
-    store_pack(reinterpret_cast<Pack<Out, VEC> *>(y + to), out);
-  };
-  for (; left >= kBatch; left -= kBatch) {
-    Pack<T, VEC> in[kBatch];
+  for (int k = 0; k < kMeans; k++) lesses[k] = UNIT > 1 ? Two(less[k], less[k]) : Two(less[2 * k], less[2 * k + 1 <= VEC ? 2 * k + 1 : 2 * k]);
 #pragma unroll
-    for (int i = 0; i < kBatch; i++) in[i] = load_last(reinterpret_cast<const Pack<T, VEC> *>(x + at + i * step));
-#pragma unroll
-    for (int i = 0; i < kBatch; i++) one(in[i], at + i * step);
-    at += kBatch * step;
+  for (int k = 0; k < kTwos; k++) {
+    gains[k] = Two(gain[2 * k], gain[2 * k + 1]);
+    shifts[k] = Two(shift[2 * k], shift[2 * k + 1]);
   }
-  Pack<T, VEC> in[kBatch - 1];
+  const int64_t first = (int64_t)row * p.channels + column * VEC, step = (int64_t)p.rows * p.channels;
+  const int act = p.act;
+  source.each([&](const auto &in, int count, int place) {
+    Out *to = y + first + place * step;
 #pragma unroll
-  for (int i = 0; i < kBatch - 1; i++)
-    if (i < left) in[i] = load_last(reinterpret_cast<const Pack<T, VEC> *>(x + at + i * step));
+    for (int i = 0; i < Source::kBatch; i++)
+      if (i < count) {
+        float v[VEC];
 #pragma unroll
-  for (int i = 0; i < kBatch - 1; i++)
-    if (i < left) one(in[i], at + i * step);
+        for (int k = 0; k < kTwos; k++) {
+          const float2 r = fma2(in[i].two(k) + lesses[k / kEach], gains[k], shifts[k]).both();
+          v[2 * k] = r.x;
+          if (2 * k + 1 < VEC) v[2 * k + (VEC > 1)] = r.y;
+        }
+        store_results(to + i * step, v, p, act);
+      }
+  });
 }
 
 __device__ __forceinline__ float2 to_stats(float2 part, float n, float eps) { return make_float2(part.x, 1.0f / sqrtf(part.y / n + eps)); }
@@ -266,10 +464,17 @@ __device__ __forceinline__ Out *result(const NormParams &p) {
   else return reinterpret_cast<Out *>(p.out);
 }
 
+// A thread's pixels of a block, by plain loads.
+template <typename T, int VEC>
+__device__ __forceinline__ Loads<T, VEC> loads_of(const T *x, int pixels, int channels, int columns, int rows) {
+  const int row = threadIdx.x / columns, column = threadIdx.x - row * columns;
+  return {x + (int64_t)row * channels + column * VEC, (int64_t)rows * channels, row < rows && row < pixels ? (pixels - row + rows - 1) / rows : 0};
+}
+
 // A block takes p.slice channels (whole groups) of one image.
 template <typename T, int VEC, int UNIT, typename Out>
 __global__ void __launch_bounds__(kNormThreads) norm_single_kernel(const NormParams p) {
-  extern __shared__ float2 norm_shared[];
+  extern __shared__ __align__(16) float2 norm_shared[];
   pdl_wait();
   pdl_launch_dependents();
   const int width = p.channels / p.groups, groups = p.slice / width;
@@ -278,50 +483,70 @@ __global__ void __launch_bounds__(kNormThreads) norm_single_kernel(const NormPar
   const T *x = reinterpret_cast<const T *>(p.in) + n * p.pixels * p.channels + c0;
   float2 *stats = norm_shared;
   const float total = (float)p.pixels * (float)width;
-  group_parts<T, VEC, UNIT>(x, (int)p.pixels, p.channels, groups, width, p.rows, norm_shared + groups,
+  const Loads<T, VEC> loads = loads_of<T, VEC>(x, (int)p.pixels, p.channels, p.slice / VEC, p.rows);
+  group_parts<T, VEC, UNIT>(loads, (int)p.pixels, groups, width, p.rows, stats + groups,
                             [&](int g, float2 part) { stats[g] = to_stats(part, total, p.eps); });
   __syncthreads();
-  normalise<T, VEC, UNIT, Out>(p, x, result<Out>(p) + n * p.pixels * p.channels + c0, (int)p.pixels, groups, width, c0, stats);
+  normalise<T, VEC, UNIT, Out>(p, loads, result<Out>(p) + n * p.pixels * p.channels + c0, groups, width, c0, stats);
 }
 
 // A block takes a chunk of one image's pixels, all channels.
 template <typename T, int VEC, int UNIT>
 __global__ void __launch_bounds__(kNormThreads) norm_stats_kernel(const NormParams p) {
-  extern __shared__ float2 norm_shared[];
+  extern __shared__ __align__(16) float2 norm_shared[];
   pdl_wait();
   pdl_launch_dependents();
   const int64_t n = blockIdx.x / p.chunks, chunk = blockIdx.x - n * p.chunks, first = chunk * p.chunk_pixels;
-  group_parts<T, VEC, UNIT>(reinterpret_cast<const T *>(p.in) + (n * p.pixels + first) * p.channels,
-                            (int)min(p.chunk_pixels, p.pixels - first), p.channels, p.groups, p.channels / p.groups, p.rows, norm_shared,
-                            [&](int g, float2 part) { p.partial[(n * p.groups + g) * p.chunks + chunk] = part; });
+  const T *x = reinterpret_cast<const T *>(p.in) + (n * p.pixels + first) * p.channels;
+  const int pixels = (int)min(p.chunk_pixels, p.pixels - first), width = p.channels / p.groups;
+  auto done = [&](int g, float2 part) { p.partial[(n * p.groups + g) * p.chunks + chunk] = part; };
+  float2 *parts = norm_shared + Stream<T, VEC>::bytes(blockDim.x) / sizeof(float2);
+  if constexpr (Stream<T, VEC>::kCan) {
+    Stream<T, VEC> stream(x, pixels, p.channels, p.rows, norm_shared, false);
+    group_parts<T, VEC, UNIT>(stream, pixels, p.groups, width, p.rows, parts, done);
+    stream.finish(p.status);
+  } else {
+    group_parts<T, VEC, UNIT>(loads_of<T, VEC>(x, pixels, p.channels, p.channels / VEC, p.rows), pixels, p.groups, width, p.rows, parts, done);
+  }
 }
 
 template <typename T, int VEC, int UNIT, typename Out>
 __global__ void __launch_bounds__(kNormThreads) norm_chunks_kernel(const NormParams p) {
-  extern __shared__ float2 norm_shared[];
+  extern __shared__ __align__(16) float2 norm_shared[];
   pdl_wait();
   pdl_launch_dependents();
   const int64_t block = gridDim.x - 1 - blockIdx.x, n = block / p.chunks, chunk = block - n * p.chunks, first = chunk * p.chunk_pixels;
-  const int width = p.channels / p.groups, lane = threadIdx.x & 31;
-  const float most = (float)p.chunk_pixels * (float)width, rest = (float)(p.pixels - (p.chunks - 1) * p.chunk_pixels) * (float)width,
-              total = (float)p.pixels * (float)width;
-  for (int g = threadIdx.x >> 5; g < p.groups; g += blockDim.x >> 5) {
-    const float2 *parts = p.partial + (n * p.groups + g) * p.chunks;
-    const float2 part = join_parts(p.chunks, total, [&](int i, float &count) {
-      count = i + 1 < p.chunks ? most : rest;
-      return parts[i];
-    });
-    if (lane == 0) norm_shared[g] = to_stats(part, total, p.eps);
-  }
-  __syncthreads();
+  const int width = p.channels / p.groups, lane = threadIdx.x & 31, pixels = (int)min(p.chunk_pixels, p.pixels - first);
   const int64_t at = (n * p.pixels + first) * p.channels;
-  normalise<T, VEC, UNIT, Out>(p, reinterpret_cast<const T *>(p.in) + at, result<Out>(p) + at, (int)min(p.chunk_pixels, p.pixels - first),
-                               p.groups, width, 0, norm_shared);
+  const T *x = reinterpret_cast<const T *>(p.in) + at;
+  float2 *stats = norm_shared + Stream<T, VEC>::bytes(blockDim.x) / sizeof(float2);
+  auto join = [&]() {
+    const float most = (float)p.chunk_pixels * (float)width, rest = (float)(p.pixels - (p.chunks - 1) * p.chunk_pixels) * (float)width,
+                total = (float)p.pixels * (float)width;
+    for (int g = threadIdx.x >> 5; g < p.groups; g += blockDim.x >> 5) {
+      const float2 *parts = p.partial + (n * p.groups + g) * p.chunks;
+      const float2 part = join_parts<10>(p.chunks, total, [&](int i, float &count) {
+        count = i + 1 < p.chunks ? most : rest;
+        return parts[i];
+      });
+      if (lane == 0) stats[g] = to_stats(part, total, p.eps);
+    }
+    __syncthreads();
+  };
+  if constexpr (Stream<T, VEC>::kCan) {
+    Stream<T, VEC> stream(x, pixels, p.channels, p.rows, norm_shared, true);
+    join();
+    normalise<T, VEC, UNIT, Out>(p, stream, result<Out>(p) + at, p.groups, width, 0, stats);
+    stream.finish(p.status);
+  } else {
+    join();
+    normalise<T, VEC, UNIT, Out>(p, loads_of<T, VEC>(x, pixels, p.channels, p.channels / VEC, p.rows), result<Out>(p) + at, p.groups, width, 0, stats);
+  }
 }
 
+// ---- any number of channels: one group to a block, a thread to an element ----
 __device__ __forceinline__ float block_sum(float v, float *shared) {
-#pragma unroll
-  for (int d = 16; d > 0; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
+  v = warp_sum(v);
   __syncthreads();
   if ((threadIdx.x & 31) == 0) shared[threadIdx.x >> 5] = v;
   __syncthreads();
@@ -330,7 +555,6 @@ __device__ __forceinline__ float block_sum(float v, float *shared) {
   return v;
 }
 
-// ---- any number of channels: one group to a block, a thread to an element ----
 // A block takes a chunk of the pixels of one group of one image.
 template <typename T>
 __global__ void __launch_bounds__(256) norm_any_parts_kernel(const NormParams p) {
@@ -382,9 +606,8 @@ __global__ void __launch_bounds__(256) norm_any_apply_kernel(const NormParams p)
     const int64_t n = i / image;
     const int c = (int)(i % p.channels);
     const float2 s = p.stats[n * p.groups + c / width];
-    float y = (to_float(reinterpret_cast<const T *>(p.in)[i]) - s.x) * s.y;
-    y = y * (p.gamma ? p.gamma[c] : 1.0f) + (p.beta ? p.beta[c] : 0.0f);
-    result<Out>(p)[i] = norm_result<Out>(y, p);
+    float y[1] = {fmaf(to_float(reinterpret_cast<const T *>(p.in)[i]) - s.x, s.y * (p.gamma ? p.gamma[c] : 1.0f), p.beta ? p.beta[c] : 0.0f)};
+    store_results(result<Out>(p) + i, y, p, p.act);
   }
 }
 
@@ -394,13 +617,22 @@ int64_t any_chunks(int64_t images, int64_t pixels, int64_t channels, int64_t gro
   const int64_t chunks = want < most ? want : most;
   return chunks < 1 ? 1 : chunks > pixels ? pixels : chunks;
 }
-// The two launches: blocks of 16 pixels to a thread or more (of 256 threads, 16 bytes of a pixel each), but as many
-// blocks as the GPU runs at once where there are pixels for them.
+// The two launches: two blocks to an SM at once, in the fewest rounds that leave few SMs idle; what a block does beside its
+// pixels takes as long as some twenty pixels to a thread do.
 int64_t image_chunks(int64_t images, int64_t pixels, int64_t channels) {
-  const int64_t rows = 2048 / channels > 1 ? 2048 / channels : 1;
-  const int64_t least = (4 * kB200Sms + images - 1) / images, by_work = pixels / (16 * rows), most = (pixels + 2 * rows - 1) / (2 * rows);
-  int64_t chunks = by_work > least ? by_work : least < most ? least : most;
-  return chunks > 256 ? 256 : chunks < 1 ? 1 : chunks;
+  const int64_t at_once = 2 * kB200Sms, rows = 2048 / channels > 1 ? 2048 / channels : 1, most = (pixels + 8 * rows - 1) / (8 * rows);
+  int64_t best = 1;
+  float used = 0.0f;
+  for (int64_t rounds = 1; rounds <= 4; rounds++) {
+    int64_t chunks = at_once * rounds / images;
+    chunks = chunks > most ? most : chunks < 1 ? 1 : chunks;
+    const float u = (float)(images * chunks) / (float)((images * chunks + at_once - 1) / at_once * at_once);
+    if (u > used + 0.04f) {
+      best = chunks;
+      used = u;
+    }
+  }
+  return best;
 }
 
 // Elements that a thread takes side by side: as many as 16 bytes hold, or four bytes, or one.
@@ -417,10 +649,9 @@ int64_t pick_slice(int64_t channels, int64_t groups, int vec, int in_bytes) {
   return 0;
 }
 
-// Threads of a block: enough for a pixel's columns; rows of them side by side, no more than there are pixels.
-int threads_for(int64_t columns) { return columns <= 128 ? 256 : kNormThreads; }
+// Pixels that a block takes side by side.
 int rows_for(int64_t columns, int64_t pixels) {
-  const int64_t rows = threads_for(columns) / columns;
+  const int64_t rows = (columns <= 256 ? 256 : kNormThreads) / columns;
   return (int)(rows < pixels ? rows : pixels);
 }
 
@@ -438,16 +669,17 @@ int launch_unit(NormParams p, int64_t slice, cudaStream_t s) {
                                 parts + (size_t)(slice / width) * sizeof(float2), s, p));
     return GLOWB200_OK;
   }
-  const dim3 grid((unsigned)(p.images * p.chunks));
-  GLOWB200_CUDA_OK(launch_pdl(norm_stats_kernel<T, VEC, UNIT>, grid, threads, parts, s, p));
-  GLOWB200_CUDA_OK(launch_pdl(norm_chunks_kernel<T, VEC, UNIT, Out>, grid, threads, (size_t)p.groups * sizeof(float2), s, p));
-  return GLOWB200_OK;
+  auto run = [&](auto kernel, size_t shared) {
+    GLOWB200_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)shared));
+    GLOWB200_CUDA_OK(launch_pdl(kernel, dim3((unsigned)(p.images * p.chunks)), threads, shared, s, p));
+    return GLOWB200_OK;
+  };
+  if (int rc = run(norm_stats_kernel<T, VEC, UNIT>, Stream<T, VEC>::bytes((int)threads) + parts)) return rc;
+  return run(norm_chunks_kernel<T, VEC, UNIT, Out>, Stream<T, VEC>::bytes((int)threads) + (size_t)p.groups * sizeof(float2));
 }
 template <typename T, int VEC, typename Out>
 int launch_vec(const NormParams &p, int64_t slice, cudaStream_t s) {
   const int width = p.channels / p.groups;
-  if constexpr (VEC == 8)
-    if (width % 8 == 0) return launch_unit<T, VEC, 8, Out>(p, slice, s);
   if constexpr (VEC >= 4)
     if (width % 4 == 0) return launch_unit<T, VEC, 4, Out>(p, slice, s);
   if constexpr (VEC >= 2)
@@ -495,7 +727,7 @@ extern "C" size_t glowb200_group_norm_workspace_bytes(int64_t images, int64_t pi
 
 extern "C" int glowb200_group_norm(void *out, int out_type, int8_t *out_i8, float quant_scale, int32_t quant_offset, const void *in, int in_type,
                                    const float *gamma, const float *beta, int64_t images, int64_t pixels, int64_t channels, int64_t groups,
-                                   float eps, int act, void *workspace, size_t workspace_bytes, glowb200_stream_t stream) {
+                                   float eps, int act, void *workspace, size_t workspace_bytes, int32_t *status, glowb200_stream_t stream) {
   GLOWB200_REQUIRE(images >= 0 && pixels >= 0 && channels > 0 && groups > 0 && images < (1ll << 31) && pixels < (1ll << 31) &&
                        channels < (1ll << 31) && images * groups < (1ll << 31),
                    "dimensions out of range");
@@ -517,7 +749,7 @@ extern "C" int glowb200_group_norm(void *out, int out_type, int8_t *out_i8, floa
   p.stats = reinterpret_cast<float2 *>(workspace);
   p.partial = reinterpret_cast<float2 *>(reinterpret_cast<uint8_t *>(workspace) + align_up((size_t)(images * groups) * 8, 256));
   p.images = images, p.pixels = pixels, p.channels = (int)channels, p.groups = (int)groups;
-  p.eps = eps, p.quant_scale = quant_scale, p.quant_offset = quant_offset, p.act = act;
+  p.eps = eps, p.quant_scale = quant_scale, p.quant_offset = quant_offset, p.act = act, p.status = status;
   GLOWB200_REQUIRE(images * groups * any_chunks(images, pixels, channels, groups) < (1ll << 31) && images * image_chunks(images, pixels, channels) < (1ll << 31),
                    "more than 2^31 groups");
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);

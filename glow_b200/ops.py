@@ -667,13 +667,13 @@ def dynamic_microscaled_fp4_fc(inp, weights, weights_scales, bias=None, *, flags
 
 
 def group_norm(x, groups, gamma=None, beta=None, eps=1e-5, *, activation=NORM_ACT_NONE, quant=None, out_dtype=None, out=None,
-               workspace=None):
+               workspace=None, status=None):
     """Group norm of channels-last activations [images, ..., channels] (float32, float16 or bfloat16) with an activation
     behind it (NORM_ACT_*); gamma, beta fp32 [channels].  Result of out_dtype, by default the input's, or int8 when
     quant=(scale, offset) (the following Quantize node fused)."""
     q = quant or (1.0, 0)
     return _native().group_norm(x, groups, gamma, beta, eps, activation, quant is not None, q[0], q[1], _float_type(out_dtype), out,
-                                workspace)
+                                workspace, status)
 
 
 def device_tensor(ptr, shape, dtype, device="cuda"):

@@ -697,7 +697,7 @@ int glowb200_dynamic_microscaled_fp4_fc(void *out, int out_type, const void *in,
 size_t glowb200_group_norm_workspace_bytes(int64_t images, int64_t pixels, int64_t channels, int64_t groups);
 int glowb200_group_norm(void *out, int out_type, int8_t *out_i8, float quant_scale, int32_t quant_offset, const void *in,
                         int in_type, const float *gamma, const float *beta, int64_t images, int64_t pixels, int64_t channels,
-                        int64_t groups, float eps, int act, void *workspace, size_t workspace_bytes,
+                        int64_t groups, float eps, int act, void *workspace, size_t workspace_bytes, int32_t *status,
                         glowb200_stream_t stream);
 
 /* ---------------------------------------------------------------------------------------

@@ -39,7 +39,7 @@ def test_nothing_to_do_needs_no_gpu(l):
     assert l.glowb200_microscaled_fp4_dequantize(None, None, 0, 64, None, 0, None) == 0
     assert l.glowb200_microscaled_fp4_fc(None, 0, None, None, None, None, None, 0, 64, 8, 0, None, None) == 0
     assert l.glowb200_dynamic_microscaled_fp4_fc(None, 0, None, 0, 64, None, None, None, 8, 64, 0, 0, None, 0, None, None) == 0
-    assert l.glowb200_group_norm(None, 0, None, 1.0, 0, None, 0, None, None, 0, 9, 8, 2, 1e-5, 0, None, 0, None) == 0
+    assert l.glowb200_group_norm(None, 0, None, 1.0, 0, None, 0, None, None, 0, 9, 8, 2, 1e-5, 0, None, 0, None, None) == 0
 
 
 @pytest.mark.parametrize("change", [dict(out_type=3), dict(K=0), dict(M=-1), dict(N=1 << 31), dict(flags=2), dict(out=None), dict(a=None),
@@ -68,7 +68,7 @@ def test_group_norm_refuses(l, change, code):
     v = dict(out=FAKE, out_type=0, out_i8=None, scale=1.0, offset=0, inp=FAKE, in_type=1, gamma=None, beta=None, images=2, pixels=9, channels=8,
              groups=2, eps=1e-5, act=0, ws=FAKE, size=1 << 20)
     v.update(change)
-    assert l.glowb200_group_norm(*v.values(), None) == code
+    assert l.glowb200_group_norm(*v.values(), None, None) == code
     assert l.glowb200_last_error()
 
 
