@@ -34,6 +34,7 @@ struct NormParams {
   int channels, groups, chunks;
   int64_t chunk_pixels;
   int slices, slice, rows;  // single launch: slices of an image, channels of one; rows: pixels that a block takes side by side
+  int held_at;              // ... where its pixels lie in shared memory
   float eps, quant_scale;
   int32_t quant_offset;
   int act;
@@ -228,6 +229,53 @@ struct Loads {
         if (first + i < left) p[i].load(at + i * step);
       at += kBatch * step;
       body(p, min(left - first, kBatch), first);
+    }
+  }
+};
+
+// The same for at most kHeld pixels of a thread that stay in shared memory, so that they come from memory once: asynchronous
+// copies of 16 bytes, four commit groups of four (each thread reads what it copied itself).
+constexpr int kHeld = 16;
+template <typename T, int VEC>
+struct Held {
+  static constexpr bool kCan = VEC * sizeof(T) == 16;
+  static constexpr int kBatch = 4;
+  __host__ __device__ static constexpr int bytes(int threads, int pixels) { return threads * 16 * pixels; }  // pixels of a thread, a multiple of 4
+  uint32_t place;
+  int left;
+  bool first;  // still on their way
+  __device__ __forceinline__ Held(const Loads<T, VEC> &from, void *shared)
+      : place((uint32_t)__cvta_generic_to_shared(shared) + 16 * threadIdx.x), left(from.left), first(true) {
+    const T *at = from.at;
+#pragma unroll
+    for (int g = 0; g < kHeld / kBatch; g++) {
+#pragma unroll
+      for (int i = 0; i < kBatch; i++)
+        if (g * kBatch + i < left) {
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(place + (g * kBatch + i) * 16 * blockDim.x), "l"(at) : "memory");
+          at += from.step;
+        }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    }
+  }
+  template <typename Body>
+  __device__ __forceinline__ void each(Body body) const {
+    Pack<T, VEC> p[kBatch];
+#pragma unroll 1
+    for (int at = 0; at < left; at += kBatch) {
+      if (first) {
+        if (at == 0) asm volatile("cp.async.wait_group 3;" ::: "memory");
+        else if (at == kBatch) asm volatile("cp.async.wait_group 2;" ::: "memory");
+        else if (at == 2 * kBatch) asm volatile("cp.async.wait_group 1;" ::: "memory");
+        else asm volatile("cp.async.wait_group 0;" ::: "memory");
+      }
+#pragma unroll
+      for (int i = 0; i < kBatch; i++)
+        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                     : "=r"(p[i].w[0]), "=r"(p[i].w[1]), "=r"(p[i].w[2]), "=r"(p[i].w[3])
+                     : "r"(place + (at + i) * 16 * blockDim.x)
+                     : "memory");  // (what is behind the last is old, and not used)
+      body(p, min(kBatch, left - at), at);
     }
   }
 };
@@ -471,23 +519,48 @@ __device__ __forceinline__ Loads<T, VEC> loads_of(const T *x, int pixels, int ch
   return {x + (int64_t)row * channels + column * VEC, (int64_t)rows * channels, row < rows && row < pixels ? (pixels - row + rows - 1) / rows : 0};
 }
 
-// A block takes p.slice channels (whole groups) of one image.
+__device__ __forceinline__ float2 ld_cluster2(uint32_t addr) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
+  return v;
+}
+
+// A cluster's blocks (one to eight) take p.slice channels (whole groups) of one image, chunk_pixels pixels each, and tell one
+// another what they know of the groups.
 template <typename T, int VEC, int UNIT, typename Out>
 __global__ void __launch_bounds__(kNormThreads) norm_single_kernel(const NormParams p) {
   extern __shared__ __align__(16) float2 norm_shared[];
   pdl_wait();
   pdl_launch_dependents();
-  const int width = p.channels / p.groups, groups = p.slice / width;
-  const int64_t n = blockIdx.x / p.slices;
-  const int c0 = (int)(blockIdx.x - n * p.slices) * p.slice;
-  const T *x = reinterpret_cast<const T *>(p.in) + n * p.pixels * p.channels + c0;
-  float2 *stats = norm_shared;
-  const float total = (float)p.pixels * (float)width;
-  const Loads<T, VEC> loads = loads_of<T, VEC>(x, (int)p.pixels, p.channels, p.slice / VEC, p.rows);
-  group_parts<T, VEC, UNIT>(loads, (int)p.pixels, groups, width, p.rows, stats + groups,
-                            [&](int g, float2 part) { stats[g] = to_stats(part, total, p.eps); });
-  __syncthreads();
-  normalise<T, VEC, UNIT, Out>(p, loads, result<Out>(p) + n * p.pixels * p.channels + c0, groups, width, c0, stats);
+  const int width = p.channels / p.groups, groups = p.slice / width, warps = blockDim.x >> 5, lane = threadIdx.x & 31;
+  const int64_t unit = blockIdx.x / p.chunks, n = unit / p.slices, first = (blockIdx.x - unit * p.chunks) * p.chunk_pixels;
+  const int c0 = (int)(unit - n * p.slices) * p.slice, pixels = (int)max((int64_t)0, min(p.chunk_pixels, p.pixels - first));
+  const int64_t at = (n * p.pixels + first) * p.channels + c0;
+  float2 *mine = norm_shared, *stats = mine + groups, *parts = stats + groups;
+  const Loads<T, VEC> loads = loads_of<T, VEC>(reinterpret_cast<const T *>(p.in) + at, pixels, p.channels, p.slice / VEC, p.rows);
+  auto run = [&](auto source) {
+    group_parts<T, VEC, UNIT>(source, pixels, groups, width, p.rows, parts, [&](int g, float2 part) { mine[g] = part; });
+    __syncthreads();
+    if (p.chunks > 1) cluster_sync();
+    const float most = (float)p.chunk_pixels * (float)width, total = (float)p.pixels * (float)width;
+    for (int g = threadIdx.x >> 5; g < groups; g += warps) {
+      const float2 part = join_parts<1>(p.chunks, total, [&](int i, float &count) {
+        const int64_t left = p.pixels - i * p.chunk_pixels;
+        count = left >= p.chunk_pixels ? most : left > 0 ? (float)left * (float)width : 0.0f;
+        if (left <= 0) return make_float2(0.0f, 0.0f);
+        return p.chunks > 1 ? ld_cluster2(map_to_cta(&mine[g], (uint32_t)i)) : mine[g];
+      });
+      if (lane == 0) stats[g] = to_stats(part, total, p.eps);
+    }
+    __syncthreads();
+    if (p.chunks > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");  // this block has read the others' parts
+    if constexpr (Held<T, VEC>::kCan) source.first = false;
+    normalise<T, VEC, UNIT, Out>(p, source, result<Out>(p) + at, groups, width, c0, stats);
+    __syncwarp();
+    if (p.chunks > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");  // none leaves before it is read
+  };
+  if constexpr (Held<T, VEC>::kCan) run(Held<T, VEC>(loads, reinterpret_cast<uint8_t *>(norm_shared) + p.held_at));
+  else run(loads);
 }
 
 // A block takes a chunk of one image's pixels, all channels.
@@ -659,14 +732,32 @@ template <typename T, int VEC, int UNIT, typename Out>
 int launch_unit(NormParams p, int64_t slice, cudaStream_t s) {
   const int width = p.channels / p.groups;
   const int64_t columns = (slice > 0 ? slice : p.channels) / VEC;
-  p.rows = rows_for(columns, slice > 0 ? p.pixels : p.chunk_pixels);
+  p.rows = rows_for(columns, p.chunk_pixels);
   const unsigned threads = (unsigned)((columns * p.rows + 31) / 32 * 32);
   const size_t parts = (size_t)(columns * p.rows * (VEC / UNIT)) * sizeof(float2);
   if (slice > 0) {
     p.slice = (int)slice;
     p.slices = (int)(p.channels / slice);
-    GLOWB200_CUDA_OK(launch_pdl(norm_single_kernel<T, VEC, UNIT, Out>, dim3((unsigned)(p.images * p.slices)), threads,
-                                parts + (size_t)(slice / width) * sizeof(float2), s, p));
+    const size_t own = parts + 2 * (size_t)(slice / width) * sizeof(float2);
+    p.held_at = (int)align_up(own, 16);
+    const int64_t each = (p.chunk_pixels + p.rows - 1) / p.rows;
+    const size_t shared = Held<T, VEC>::kCan ? p.held_at + Held<T, VEC>::bytes((int)threads, (int)align_up((size_t)each, 4)) : own;
+    auto kernel = norm_single_kernel<T, VEC, UNIT, Out>;
+    GLOWB200_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)shared));
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(p.images * p.slices * p.chunks));
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = shared;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)p.chunks;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = pdl_enabled() ? 2 : 1;
+    GLOWB200_CUDA_OK(cudaLaunchKernelEx(&cfg, kernel, static_cast<const NormParams>(p)));
     return GLOWB200_OK;
   }
   auto run = [&](auto kernel, size_t shared) {
@@ -688,20 +779,33 @@ int launch_vec(const NormParams &p, int64_t slice, cudaStream_t s) {
 }
 
 template <typename T, typename Out>
+int launch_width(const NormParams &p, int vec, int64_t slice, cudaStream_t s) {
+  if (vec == 1) return launch_vec<T, 1, Out>(p, slice, s);
+  if constexpr (sizeof(T) == 4) return launch_vec<T, 4, Out>(p, slice, s);
+  else return vec == 8 ? launch_vec<T, 8, Out>(p, slice, s) : launch_vec<T, 2, Out>(p, slice, s);
+}
+
+template <typename T, typename Out>
 int launch(NormParams p, cudaStream_t s) {
   const void *out = sizeof(Out) == 1 ? static_cast<const void *>(p.out_i8) : p.out;
   const int vec = side_by_side(p.in, out, sizeof(T), sizeof(Out), p.channels);
   int64_t slice = pick_slice(p.channels, p.groups, vec, sizeof(T));
-  const char *e = getenv("GN_MODE");
-  const bool single = slice > 0 && (e ? e[0] == 's' : p.pixels * slice * (int64_t)sizeof(T) <= 65536);
-  if (single || p.channels / vec <= kNormThreads) {
+  if (slice > 0) {  // ... over as few blocks as hold its pixels, eight at most
+    const int64_t rows = rows_for(slice / vec, p.pixels), most = rows * (kHeld - 1);
+    int64_t blocks = 1;
+    while (blocks < 8 && blocks * most < p.pixels) blocks *= 2;
+    const char *e = getenv("GN_MODE");
+    if (blocks * most >= p.pixels && !(e && e[0] == 't')) {
+      p.chunks = (int)blocks;
+      p.chunk_pixels = (p.pixels + blocks - 1) / blocks;
+      return launch_width<T, Out>(p, vec, slice, s);
+    }
+  }
+  if (p.channels / vec <= kNormThreads) {
     const int64_t chunks = image_chunks(p.images, p.pixels, p.channels);
     p.chunk_pixels = (p.pixels + chunks - 1) / chunks;
     p.chunks = (int)((p.pixels + p.chunk_pixels - 1) / p.chunk_pixels);
-    if (!single) slice = 0;
-    if (vec == 1) return launch_vec<T, 1, Out>(p, slice, s);
-    if constexpr (sizeof(T) == 4) return launch_vec<T, 4, Out>(p, slice, s);
-    else return vec == 8 ? launch_vec<T, 8, Out>(p, slice, s) : launch_vec<T, 2, Out>(p, slice, s);
+    return launch_width<T, Out>(p, vec, 0, s);
   }
   const int64_t chunks = any_chunks(p.images, p.pixels, p.channels, p.groups), blocks = (p.images * p.pixels * p.channels + 255) / 256;
   p.chunk_pixels = (p.pixels + chunks - 1) / chunks;
