@@ -12,8 +12,6 @@
 // pixels twice, the second time from cache.  Others take two: statistics of chunks of pixels, all channels to a block, then
 // a pass that joins them and normalises, from the last chunk to the first: what the first pass read last is still in L2
 // (126 MB).
-#include <cstdlib>
-
 #include "microscaled.cuh"
 #include "tcgen05.cuh"
 
@@ -35,6 +33,8 @@ struct NormParams {
   int64_t chunk_pixels;
   int slices, slice, rows;  // single launch: slices of an image, channels of one; rows: pixels that a block takes side by side
   int held_at;              // ... where its pixels lie in shared memory
+  int width, columns, of_group;  // channels of a group; pieces of a pixel that a block takes; units of a group
+  uint32_t by_width, by_columns, by_rows, by_group;  // (for fast_div)
   float eps, quant_scale;
   int32_t quant_offset;
   int act;
@@ -212,6 +212,18 @@ __device__ __forceinline__ void store_results(Out *p, float (&y)[VEC], const Nor
   }
 }
 
+// Which pixels of a block are this thread's: every rows-th from `row` on, in the column's channels.
+struct Place {
+  int row, column, base, extra;  // row r has `base` pixels, the first `extra` rows one more
+  __device__ __forceinline__ Place(const NormParams &p, int pixels) {
+    row = fast_div((int)threadIdx.x, p.columns, p.by_columns);
+    column = (int)threadIdx.x - row * p.columns;
+    base = fast_div(pixels, p.rows, p.by_rows);
+    extra = pixels - base * p.rows;
+  }
+  __device__ __forceinline__ int pixels(const NormParams &p) const { return row < p.rows ? base + (row < extra ? 1 : 0) : 0; }
+};
+
 // A block's pixels by plain loads: calls body(pixels, how many, the first one's place) for those of this thread, `left` from
 // `at` on.
 template <typename T, int VEC>
@@ -293,7 +305,7 @@ struct Stream {
   uint8_t *ring;
   uint64_t *full, *empty;
   volatile int *gave_up;
-  int pixels, rows, stages, stage_bytes;
+  int pixels, rows, columns, mine, stages, stage_bytes;  // mine: pixels of this thread
   uint32_t pixel_bytes;
   bool backwards;  // from the last stage to the first
 
@@ -307,10 +319,10 @@ struct Stream {
                  : "memory");
   }
   // By all threads: barriers, and the first stages on their way.
-  __device__ __forceinline__ Stream(const T *from, int pixels, int channels, int rows, void *shared, bool backwards)
-      : x(reinterpret_cast<const uint8_t *>(from)), ring(reinterpret_cast<uint8_t *>(shared)), pixels(pixels), rows(rows),
-        stages((pixels + kBatch * rows - 1) / (kBatch * rows)), stage_bytes(blockDim.x * 16 * kBatch),
-        pixel_bytes(channels * (uint32_t)sizeof(T)), backwards(backwards) {
+  __device__ __forceinline__ Stream(const NormParams &p, const T *from, int pixels, const Place &place, void *shared, bool backwards)
+      : x(reinterpret_cast<const uint8_t *>(from)), ring(reinterpret_cast<uint8_t *>(shared)), pixels(pixels), rows(p.rows), columns(p.columns),
+        mine(place.pixels(p)), stages((place.base + (place.extra ? 1 : 0) + kBatch - 1) / kBatch), stage_bytes(blockDim.x * 16 * kBatch),
+        pixel_bytes(p.channels * (uint32_t)sizeof(T)), backwards(backwards) {
     full = reinterpret_cast<uint64_t *>(ring + kStages * stage_bytes);
     empty = full + kStages;
     gave_up = reinterpret_cast<volatile int *>(empty + kStages);
@@ -328,8 +340,7 @@ struct Stream {
   // body(pixels, how many, the first one's place among this thread's)
   template <typename Body>
   __device__ __forceinline__ void each(Body body) {
-    const int t = threadIdx.x, columns = (int)(pixel_bytes >> 4), row = t / columns;
-    const int mine = row < rows && row < pixels ? (pixels - row + rows - 1) / rows : 0;  // pixels of this thread
+    const int t = threadIdx.x;
     const uint32_t place = smem_u32(ring) + 16 * t, apart = 16 * rows * columns;
     int slot = 0;
     uint32_t round = 0;
@@ -383,18 +394,18 @@ struct Stream {
 // Statistics of `groups` groups of `width` channels over `pixels` pixels, which `source` hands out.  Thread t of the first columns * rows has VEC channels (column t % columns) of every
 // rows-th pixel; UNIT: how many neighbours of them lie in one group.  Lane 0 of the warp that gets a group calls done(group, {mean, M2}).
 template <typename T, int VEC, int UNIT, typename Source, typename Done>
-__device__ __forceinline__ void group_parts(Source source, int pixels, int groups, int width, int rows, float2 *shared, Done done) {
+__device__ __forceinline__ void group_parts(const NormParams &p, Source source, int pixels, const Place &place, int groups, float2 *shared,
+                                            Done done) {
   // A unit's numbers are one sum; units of one channel come two to a register pair.
   constexpr int kBatch = Source::kBatch, kUnits = VEC / UNIT, kTwos = Pack<T, VEC>::kTwos, kSums = UNIT > 1 ? kUnits : kTwos, kEach = UNIT > 1 ? UNIT / 2 : 1;
-  const int columns = groups * width / VEC, t = threadIdx.x, row = t / columns;
-  const int base = pixels / rows, extra = pixels - base * rows;  // row r has base pixels, the first `extra` rows one more
+  const int t = threadIdx.x;
   {
     Two mean[kSums], squares[kSums];  // (UNIT > 1: both halves of a mean are the same, those of M2 are to be added)
     float n = 0.0f;
 #pragma unroll
     for (int k = 0; k < kSums; k++) mean[k] = squares[k] = Two(0.0f, 0.0f);
     // `count` of kBatch pixels: their mean, the squares of what they differ from it, and those joined to what was before.
-    auto take = [&](const auto &p, auto count) {
+    auto take = [&](const auto &from, auto count) {
       const float many = (float)count, numbers = many * (float)UNIT;
       const float each = decltype(count)::value ? 1.0f / (float)(decltype(count)::value * UNIT) : __fdividef(1.0f, numbers);
       const float share = __fdividef(many, n + many), cross = (UNIT > 1 ? 0.5f : 1.0f) * n * share * (float)UNIT;
@@ -407,7 +418,7 @@ __device__ __forceinline__ void group_parts(Source source, int pixels, int group
           if (i < count) {
 #pragma unroll
             for (int k = 0; k < kEach; k++) {
-              x[i][k] = p[i].two(u * kEach + k);
+              x[i][k] = from[i].two(u * kEach + k);
               sum = i == 0 && k == 0 ? x[i][k] : sum + x[i][k];
             }
           }
@@ -428,11 +439,11 @@ __device__ __forceinline__ void group_parts(Source source, int pixels, int group
       }
       n += many;
     };
-    source.each([&](const auto &p, int count, int) {
-      if (count == kBatch) take(p, Known<kBatch>());
-      else take(p, Count{count});
+    source.each([&](const auto &x, int count, int) {
+      if (count == kBatch) take(x, Known<kBatch>());
+      else take(x, Count{count});
     });
-    if (row < rows)
+    if (place.row < p.rows)
 #pragma unroll
     for (int u = 0; u < kSums; u++) {
       const float2 m = mean[u].both(), q = squares[u].both();
@@ -445,14 +456,13 @@ __device__ __forceinline__ void group_parts(Source source, int pixels, int group
     }
   }
   __syncthreads();
-  const int per_row = columns * kUnits, of_group = width / UNIT, warps = blockDim.x >> 5, lane = t & 31;
-  const uint32_t reciprocal = 0xffffffffu / (uint32_t)of_group;
-  const float few = (float)base * (float)UNIT, many = (float)(base + 1) * (float)UNIT, total = (float)pixels * (float)width;
+  const int per_row = p.columns * kUnits, warps = blockDim.x >> 5, lane = t & 31;
+  const float few = (float)place.base * (float)UNIT, many = (float)(place.base + 1) * (float)UNIT, total = (float)pixels * (float)p.width;
   for (int g = t >> 5; g < groups; g += warps) {
-    const float2 part = join_parts<4>(rows * of_group, total, [&](int i, float &n) {  // units of the group, row by row
-      const int r = fast_div(i, of_group, reciprocal);
-      n = r < extra ? many : few;
-      return shared[r * per_row + g * of_group + (i - r * of_group)];
+    const float2 part = join_parts<4>(p.rows * p.of_group, total, [&](int i, float &n) {  // units of the group, row by row
+      const int r = fast_div(i, p.of_group, p.by_group);
+      n = r < place.extra ? many : few;
+      return shared[r * per_row + g * p.of_group + (i - r * p.of_group)];
     });
     if (lane == 0) done(g, part);
   }
@@ -460,16 +470,16 @@ __device__ __forceinline__ void group_parts(Source source, int pixels, int group
 
 // Normalises the same pixels; stats: mean and 1 / sqrt(var + eps) of the groups; c0: their first channel.
 template <typename T, int VEC, int UNIT, typename Out, typename Source>
-__device__ __forceinline__ void normalise(const NormParams &p, Source source, Out *y, int groups, int width, int c0, const float2 *stats) {
+__device__ __forceinline__ void normalise(const NormParams &p, Source source, Out *y, const Place &place, int c0, const float2 *stats) {
   constexpr int kTwos = Pack<T, VEC>::kTwos;
-  const int columns = groups * width / VEC, t = threadIdx.x, row = t / columns, column = t - row * columns;
+  const int column = place.column;
   // (x - mean) * gain + shift, the difference first: where a group's numbers hardly differ, gains are large
   constexpr int kMeans = UNIT > 1 ? VEC / UNIT : kTwos, kEach = UNIT > 1 ? UNIT / 2 : 1;  // of register pairs
   float less[VEC / UNIT + 1] = {}, gain[2 * kTwos] = {}, shift[2 * kTwos] = {};
-  if (row < p.rows)
+  if (place.row < p.rows)
 #pragma unroll
   for (int u = 0; u < VEC; u += UNIT) {
-    const float2 s = stats[(column * VEC + u) / width];
+    const float2 s = stats[fast_div(column * VEC + u, p.width, p.by_width)];
     less[u / UNIT] = -s.x;
 #pragma unroll
     for (int k = u; k < u + UNIT; k++) {
@@ -486,10 +496,10 @@ __device__ __forceinline__ void normalise(const NormParams &p, Source source, Ou
     gains[k] = Two(gain[2 * k], gain[2 * k + 1]);
     shifts[k] = Two(shift[2 * k], shift[2 * k + 1]);
   }
-  const int64_t first = (int64_t)row * p.channels + column * VEC, step = (int64_t)p.rows * p.channels;
+  const int64_t first = (int64_t)place.row * p.channels + column * VEC, step = (int64_t)p.rows * p.channels;
   const int act = p.act;
-  source.each([&](const auto &in, int count, int place) {
-    Out *to = y + first + place * step;
+  source.each([&](const auto &in, int count, int from) {
+    Out *to = y + first + from * step;
 #pragma unroll
     for (int i = 0; i < Source::kBatch; i++)
       if (i < count) {
@@ -514,9 +524,8 @@ __device__ __forceinline__ Out *result(const NormParams &p) {
 
 // A thread's pixels of a block, by plain loads.
 template <typename T, int VEC>
-__device__ __forceinline__ Loads<T, VEC> loads_of(const T *x, int pixels, int channels, int columns, int rows) {
-  const int row = threadIdx.x / columns, column = threadIdx.x - row * columns;
-  return {x + (int64_t)row * channels + column * VEC, (int64_t)rows * channels, row < rows && row < pixels ? (pixels - row + rows - 1) / rows : 0};
+__device__ __forceinline__ Loads<T, VEC> loads_of(const NormParams &p, const T *x, const Place &place) {
+  return {x + (int64_t)place.row * p.channels + place.column * VEC, (int64_t)p.rows * p.channels, place.pixels(p)};
 }
 
 __device__ __forceinline__ float2 ld_cluster2(uint32_t addr) {
@@ -532,14 +541,16 @@ __global__ void __launch_bounds__(kNormThreads) norm_single_kernel(const NormPar
   extern __shared__ __align__(16) float2 norm_shared[];
   pdl_wait();
   pdl_launch_dependents();
-  const int width = p.channels / p.groups, groups = p.slice / width, warps = blockDim.x >> 5, lane = threadIdx.x & 31;
-  const int64_t unit = blockIdx.x / p.chunks, n = unit / p.slices, first = (blockIdx.x - unit * p.chunks) * p.chunk_pixels;
+  const int width = p.width, groups = fast_div(p.slice, width, p.by_width), warps = blockDim.x >> 5, lane = threadIdx.x & 31;
+  const unsigned unit = blockIdx.x / (unsigned)p.chunks, n = unit / (unsigned)p.slices;
+  const int64_t first = (int64_t)(blockIdx.x - unit * p.chunks) * p.chunk_pixels;
   const int c0 = (int)(unit - n * p.slices) * p.slice, pixels = (int)max((int64_t)0, min(p.chunk_pixels, p.pixels - first));
-  const int64_t at = (n * p.pixels + first) * p.channels + c0;
+  const int64_t at = ((int64_t)n * p.pixels + first) * p.channels + c0;
+  const Place place(p, pixels);
   float2 *mine = norm_shared, *stats = mine + groups, *parts = stats + groups;
-  const Loads<T, VEC> loads = loads_of<T, VEC>(reinterpret_cast<const T *>(p.in) + at, pixels, p.channels, p.slice / VEC, p.rows);
+  const Loads<T, VEC> loads = loads_of<T, VEC>(p, reinterpret_cast<const T *>(p.in) + at, place);
   auto run = [&](auto source) {
-    group_parts<T, VEC, UNIT>(source, pixels, groups, width, p.rows, parts, [&](int g, float2 part) { mine[g] = part; });
+    group_parts<T, VEC, UNIT>(p, source, pixels, place, groups, parts, [&](int g, float2 part) { mine[g] = part; });
     __syncthreads();
     if (p.chunks > 1) cluster_sync();
     const float most = (float)p.chunk_pixels * (float)width, total = (float)p.pixels * (float)width;
@@ -553,11 +564,11 @@ __global__ void __launch_bounds__(kNormThreads) norm_single_kernel(const NormPar
       if (lane == 0) stats[g] = to_stats(part, total, p.eps);
     }
     __syncthreads();
-    if (p.chunks > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");  // this block has read the others' parts
+    if (p.chunks > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");  // this block has read the others' parts
     if constexpr (Held<T, VEC>::kCan) source.first = false;
-    normalise<T, VEC, UNIT, Out>(p, source, result<Out>(p) + at, groups, width, c0, stats);
+    normalise<T, VEC, UNIT, Out>(p, source, result<Out>(p) + at, place, c0, stats);
     __syncwarp();
-    if (p.chunks > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");  // none leaves before it is read
+    if (p.chunks > 1) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");  // none leaves before it is read
   };
   if constexpr (Held<T, VEC>::kCan) run(Held<T, VEC>(loads, reinterpret_cast<uint8_t *>(norm_shared) + p.held_at));
   else run(loads);
@@ -569,17 +580,18 @@ __global__ void __launch_bounds__(kNormThreads) norm_stats_kernel(const NormPara
   extern __shared__ __align__(16) float2 norm_shared[];
   pdl_wait();
   pdl_launch_dependents();
-  const int64_t n = blockIdx.x / p.chunks, chunk = blockIdx.x - n * p.chunks, first = chunk * p.chunk_pixels;
+  const int64_t n = blockIdx.x / (unsigned)p.chunks, chunk = blockIdx.x - n * p.chunks, first = chunk * p.chunk_pixels;
   const T *x = reinterpret_cast<const T *>(p.in) + (n * p.pixels + first) * p.channels;
-  const int pixels = (int)min(p.chunk_pixels, p.pixels - first), width = p.channels / p.groups;
+  const int pixels = (int)min(p.chunk_pixels, p.pixels - first);
+  const Place place(p, pixels);
   auto done = [&](int g, float2 part) { p.partial[(n * p.groups + g) * p.chunks + chunk] = part; };
   float2 *parts = norm_shared + Stream<T, VEC>::bytes(blockDim.x) / sizeof(float2);
   if constexpr (Stream<T, VEC>::kCan) {
-    Stream<T, VEC> stream(x, pixels, p.channels, p.rows, norm_shared, false);
-    group_parts<T, VEC, UNIT>(stream, pixels, p.groups, width, p.rows, parts, done);
+    Stream<T, VEC> stream(p, x, pixels, place, norm_shared, false);
+    group_parts<T, VEC, UNIT>(p, stream, pixels, place, p.groups, parts, done);
     stream.finish(p.status);
   } else {
-    group_parts<T, VEC, UNIT>(loads_of<T, VEC>(x, pixels, p.channels, p.channels / VEC, p.rows), pixels, p.groups, width, p.rows, parts, done);
+    group_parts<T, VEC, UNIT>(p, loads_of<T, VEC>(p, x, place), pixels, place, p.groups, parts, done);
   }
 }
 
@@ -588,10 +600,12 @@ __global__ void __launch_bounds__(kNormThreads) norm_chunks_kernel(const NormPar
   extern __shared__ __align__(16) float2 norm_shared[];
   pdl_wait();
   pdl_launch_dependents();
-  const int64_t block = gridDim.x - 1 - blockIdx.x, n = block / p.chunks, chunk = block - n * p.chunks, first = chunk * p.chunk_pixels;
-  const int width = p.channels / p.groups, lane = threadIdx.x & 31, pixels = (int)min(p.chunk_pixels, p.pixels - first);
+  const unsigned block = gridDim.x - 1 - blockIdx.x;
+  const int64_t n = block / (unsigned)p.chunks, chunk = block - n * p.chunks, first = chunk * p.chunk_pixels;
+  const int width = p.width, lane = threadIdx.x & 31, pixels = (int)min(p.chunk_pixels, p.pixels - first);
   const int64_t at = (n * p.pixels + first) * p.channels;
   const T *x = reinterpret_cast<const T *>(p.in) + at;
+  const Place place(p, pixels);
   float2 *stats = norm_shared + Stream<T, VEC>::bytes(blockDim.x) / sizeof(float2);
   auto join = [&]() {
     const float most = (float)p.chunk_pixels * (float)width, rest = (float)(p.pixels - (p.chunks - 1) * p.chunk_pixels) * (float)width,
@@ -607,13 +621,13 @@ __global__ void __launch_bounds__(kNormThreads) norm_chunks_kernel(const NormPar
     __syncthreads();
   };
   if constexpr (Stream<T, VEC>::kCan) {
-    Stream<T, VEC> stream(x, pixels, p.channels, p.rows, norm_shared, true);
+    Stream<T, VEC> stream(p, x, pixels, place, norm_shared, true);
     join();
-    normalise<T, VEC, UNIT, Out>(p, stream, result<Out>(p) + at, p.groups, width, 0, stats);
+    normalise<T, VEC, UNIT, Out>(p, stream, result<Out>(p) + at, place, 0, stats);
     stream.finish(p.status);
   } else {
     join();
-    normalise<T, VEC, UNIT, Out>(p, loads_of<T, VEC>(x, pixels, p.channels, p.channels / VEC, p.rows), result<Out>(p) + at, p.groups, width, 0, stats);
+    normalise<T, VEC, UNIT, Out>(p, loads_of<T, VEC>(p, x, place), result<Out>(p) + at, place, 0, stats);
   }
 }
 
@@ -733,6 +747,9 @@ int launch_unit(NormParams p, int64_t slice, cudaStream_t s) {
   const int width = p.channels / p.groups;
   const int64_t columns = (slice > 0 ? slice : p.channels) / VEC;
   p.rows = rows_for(columns, p.chunk_pixels);
+  auto reciprocal = [](int64_t d) { return 0xffffffffu / (uint32_t)d; };
+  p.width = width, p.columns = (int)columns, p.of_group = width / UNIT;
+  p.by_width = reciprocal(width), p.by_columns = reciprocal(columns), p.by_rows = reciprocal(p.rows), p.by_group = reciprocal(p.of_group);
   const unsigned threads = (unsigned)((columns * p.rows + 31) / 32 * 32);
   const size_t parts = (size_t)(columns * p.rows * (VEC / UNIT)) * sizeof(float2);
   if (slice > 0) {
@@ -794,8 +811,7 @@ int launch(NormParams p, cudaStream_t s) {
     const int64_t rows = rows_for(slice / vec, p.pixels), most = rows * (kHeld - 1);
     int64_t blocks = 1;
     while (blocks < 8 && blocks * most < p.pixels) blocks *= 2;
-    const char *e = getenv("GN_MODE");
-    if (blocks * most >= p.pixels && !(e && e[0] == 't')) {
+    if (blocks * most >= p.pixels) {
       p.chunks = (int)blocks;
       p.chunk_pixels = (p.pixels + blocks - 1) / blocks;
       return launch_width<T, Out>(p, vec, slice, s);

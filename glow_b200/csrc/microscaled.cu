@@ -8,34 +8,86 @@
 namespace glowb200 {
 namespace {
 
-constexpr int kQuantThreads = 256;
+constexpr int kThreads = 256;
 
-// A block takes a scale tile: 128 rows by 128 columns.  Eight neighbours of a row to a lane, so four lanes share a scale;
-// a warp has two rows at a time.
-template <typename T, bool VEC>
-__global__ void __launch_bounds__(kQuantThreads) mx_quantize_kernel(const T *__restrict__ in, int64_t rows, int64_t cols, int64_t row_stride,
-                                                                    int64_t tiles, uint8_t *__restrict__ data, uint8_t *__restrict__ scales) {
+// Both kernels: a block takes a scale tile, 128 rows by 128 columns; eight neighbours of a row to a lane, so four lanes share
+// a scale, a warp has two rows at a time and a thread eight places.  All of a thread's loads are asked for before the
+// first is used.
+struct TilePlace {
+  int64_t row0, col;  // of the block; of the thread's eight columns
+  int first, rows;    // the thread's first row of the block; rows that are there
+  __device__ __forceinline__ TilePlace(int64_t all_rows, unsigned tiles) {
+    const unsigned row_tile = blockIdx.x / tiles;
+    row0 = (int64_t)row_tile * 128;
+    col = (int64_t)(blockIdx.x - row_tile * tiles) * 128 + (threadIdx.x & 15) * 8;
+    first = (int)(threadIdx.x >> 4);
+    rows = (int)min((int64_t)128, all_rows - row0);
+  }
+};
+
+// RAGGED: rows off 16-byte boundaries, or whose last eight columns are not all there.  Their elements come one to a lane, 32
+// neighbours at a time, and change places in shared memory: eight single loads to a lane would ask for eight times as
+// many lines.
+template <typename T, bool RAGGED>
+__global__ void __launch_bounds__(kThreads) mx_quantize_kernel(const T *__restrict__ in, int64_t rows, int64_t cols, int64_t row_stride,
+                                                               unsigned tiles, uint8_t *__restrict__ data, uint8_t *__restrict__ scales) {
   __shared__ __align__(16) uint8_t tile[512];
+  __shared__ __align__(16) T staged[RAGGED ? kThreads * 8 : 8];
   pdl_wait();
   pdl_launch_dependents();
-  const int64_t row_tile = blockIdx.x / tiles, col_tile = blockIdx.x - row_tile * tiles;
+  const TilePlace at(rows, tiles);
+  const int lane = threadIdx.x & 31;
   if (threadIdx.x < 32) reinterpret_cast<uint4 *>(tile)[threadIdx.x] = make_uint4(0, 0, 0, 0);
   __syncthreads();
-  const int lane = threadIdx.x & 31, first = threadIdx.x >> 4;  // 16 threads to a row
-  const int64_t col = col_tile * 128 + (lane & 15) * 8, pitch = 16 * ((cols + 31) / 32);
-#pragma unroll 4
-  for (int i = 0; i < 8; i++) {
-    const int r = i * 16 + first;
-    const int64_t row = row_tile * 128 + r;
-    if (row_tile * 128 + i * 16 + (first & ~1) >= rows) break;  // (of the warp's two rows the first: all lanes leave together)
-    const bool real = row < rows;
-    Eight<VEC, T> x;
-    x.load(in + row * row_stride + col, real ? cols - col : 0);
+  const int64_t pitch = 16 * ((cols + 31) / 32);
+  const T *x = in + (at.row0 + at.first) * row_stride + at.col;
+  const int64_t left = cols - at.col;
+  auto finish = [&](int i, const Eight<true, T> &v) {
+    const int r = i * 16 + at.first;
     uint32_t byte;
-    const uint32_t codes = mx_block(x, byte);
-    if (real && col / 2 < pitch) {  // (pitch: whole blocks)
-      *reinterpret_cast<uint32_t *>(data + row * pitch + col / 2) = codes;
+    const uint32_t codes = mx_block(v, byte);
+    if (r < at.rows && at.col / 2 < pitch) {  // (pitch: whole blocks)
+      *reinterpret_cast<uint32_t *>(data + (at.row0 + r) * pitch + at.col / 2) = codes;
       if ((lane & 3) == 0) tile[(r & 31) * 16 + (r >> 5) * 4 + ((lane & 15) >> 2)] = (uint8_t)byte;
+    }
+  };
+  constexpr int kAtOnce = sizeof(T) == 4 ? 4 : 8;
+#pragma unroll
+  for (int i0 = 0; i0 < 8; i0 += kAtOnce) {
+    if (i0 * 16 >= at.rows) break;
+    Eight<true, T> v[kAtOnce];
+    if constexpr (!RAGGED) {
+#pragma unroll
+      for (int i = 0; i < kAtOnce; i++) v[i].load(x + (int64_t)(i0 + i) * 16 * row_stride, (i0 + i) * 16 + at.first < at.rows ? left : 0);
+#pragma unroll
+      for (int i = 0; i < kAtOnce; i++)
+        if ((i0 + i) * 16 < at.rows) finish(i0 + i, v[i]);
+    } else {
+      // the warp's two rows of 128 columns, 32 at a time: element e of them is row e / 128, column e % 128
+      T *mine = staged + (threadIdx.x & ~31) * 8;
+      const int64_t col0 = at.col - (lane & 15) * 8;
+      const int row = (at.first & ~1);
+      T w[kAtOnce][8];
+#pragma unroll
+      for (int i = 0; i < kAtOnce; i++)
+#pragma unroll
+        for (int k = 0; k < 8; k++) {
+          const int r = (i0 + i) * 16 + row + (k >> 2);
+          const int64_t c = col0 + (k & 3) * 32 + lane;
+          w[i][k] = r < at.rows && c < cols ? in[(at.row0 + r) * row_stride + c] : from_float<T>(0.0f);
+        }
+#pragma unroll
+      for (int i = 0; i < kAtOnce; i++)
+        if ((i0 + i) * 16 < at.rows) {
+          __syncwarp();
+#pragma unroll
+          for (int k = 0; k < 8; k++) mine[k * 32 + lane] = w[i][k];
+          __syncwarp();
+#pragma unroll
+          for (int k = 0; k < (int)(8 * sizeof(T) / 16); k++)
+            reinterpret_cast<uint4 *>(v[i].w)[k] = reinterpret_cast<const uint4 *>(mine + lane * 8)[k];
+          finish(i0 + i, v[i]);
+        }
     }
   }
   __syncthreads();
@@ -43,31 +95,63 @@ __global__ void __launch_bounds__(kQuantThreads) mx_quantize_kernel(const T *__r
     reinterpret_cast<uint4 *>(scales + (size_t)blockIdx.x * 512)[threadIdx.x] = reinterpret_cast<const uint4 *>(tile)[threadIdx.x];
 }
 
-template <typename T, bool VEC>
-__global__ void __launch_bounds__(256) mx_dequantize_kernel(const uint8_t *__restrict__ data, const uint8_t *__restrict__ scales, int64_t rows,
-                                                            int64_t cols, int64_t tiles, T *__restrict__ out) {
+template <typename T, bool RAGGED>
+__global__ void __launch_bounds__(kThreads) mx_dequantize_kernel(const uint8_t *__restrict__ data, const uint8_t *__restrict__ scales, int64_t rows,
+                                                                 int64_t cols, unsigned tiles, T *__restrict__ out) {
+  __shared__ __align__(16) uint8_t tile[512];
+  __shared__ __align__(16) T staged[RAGGED ? kThreads * 8 : 8];
   pdl_wait();
   pdl_launch_dependents();
-  const int64_t chunks = (cols + 7) / 8, pitch = 16 * ((cols + 31) / 32);
-  for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < rows * chunks; i += gridDim.x * 256ll) {
-    const int64_t row = i / chunks, col = (i - row * chunks) * 8;
-    const uint32_t codes = *reinterpret_cast<const uint32_t *>(data + row * pitch + col / 2);
-    const float scale = mx_scale(scales[mx_scale_at(row, col >> 5, tiles)]);
-    __align__(16) T w[8];
+  const TilePlace at(rows, tiles);
+  const int lane = threadIdx.x & 31;
+  const int64_t pitch = 16 * ((cols + 31) / 32);
+  const uint8_t *d = data + (at.row0 + at.first) * pitch + at.col / 2;
+  uint32_t codes[8];
+#pragma unroll
+  for (int i = 0; i < 8; i++)
+    codes[i] = i * 16 + at.first < at.rows && at.col < cols ? __ldg(reinterpret_cast<const uint32_t *>(d + (int64_t)i * 16 * pitch)) : 0u;
+  if (threadIdx.x < 32)
+    reinterpret_cast<uint4 *>(tile)[threadIdx.x] = __ldg(reinterpret_cast<const uint4 *>(scales + (size_t)blockIdx.x * 512) + threadIdx.x);
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 8; i++) {
+    if (i * 16 >= at.rows) break;
+    const int r = i * 16 + at.first;
+    const float scale = mx_scale(tile[(r & 31) * 16 + (r >> 5) * 4 + ((lane & 15) >> 2)]);
+    float v[8];
 #pragma unroll
     for (int k = 0; k < 4; k++) {
-      const float2 n = mx_numbers((codes >> (8 * k)) & 0xFFu);
-      w[2 * k] = from_float<T>(n.x * scale);
-      w[2 * k + 1] = from_float<T>(n.y * scale);
+      const float2 n = mx_numbers((codes[i] >> (8 * k)) & 0xFFu);
+      v[2 * k] = n.x * scale;
+      v[2 * k + 1] = n.y * scale;
     }
-    T *o = out + row * cols + col;
-    if (VEC) {
+    uint32_t w[2 * sizeof(T)];
 #pragma unroll
-      for (int k = 0; k < (int)(8 * sizeof(T) / 16); k++) reinterpret_cast<uint4 *>(o)[k] = reinterpret_cast<const uint4 *>(w)[k];
+    for (int k = 0; k < (int)(2 * sizeof(T)); k++) {
+      if constexpr (sizeof(T) == 4) w[k] = __float_as_uint(v[k]);
+      else w[k] = pack2(v[2 * k], v[2 * k + 1], T());
+    }
+    if constexpr (!RAGGED) {
+      if (r < at.rows && at.col < cols) {
+        T *o = out + (at.row0 + r) * cols + at.col;
+#pragma unroll
+        for (int k = 0; k < (int)(sizeof(T) / 2); k++)
+          reinterpret_cast<uint4 *>(o)[k] = make_uint4(w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]);
+      }
     } else {
+      T *mine = staged + (threadIdx.x & ~31) * 8;
+      __syncwarp();
 #pragma unroll
-      for (int k = 0; k < 8; k++)
-        if (col + k < cols) o[k] = w[k];
+      for (int k = 0; k < (int)(sizeof(T) / 2); k++)
+        reinterpret_cast<uint4 *>(mine + lane * 8)[k] = make_uint4(w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]);
+      __syncwarp();
+      const int64_t col0 = at.col - (lane & 15) * 8;
+#pragma unroll
+      for (int k = 0; k < 8; k++) {
+        const int rr = i * 16 + (at.first & ~1) + (k >> 2);
+        const int64_t c = col0 + (k & 3) * 32 + lane;
+        if (rr < at.rows && c < cols) out[(at.row0 + rr) * cols + c] = mine[k * 32 + lane];
+      }
     }
   }
 }
@@ -85,10 +169,10 @@ int run_mx_quantize(const void *in, int in_type, int64_t rows, int64_t cols, int
   GLOWB200_REQUIRE(blocks < (1ll << 31), "the matrix has more than 2^31 tiles of 128 x 128");
   return with_float_type(in_type, [&](auto *t) {
     using T = std::remove_pointer_t<decltype(t)>;
-    const bool vec = aligned(in, 16) && (row_stride * sizeof(T)) % 16 == 0;
-    auto kernel = vec ? mx_quantize_kernel<T, true> : mx_quantize_kernel<T, false>;
-    GLOWB200_CUDA_OK(launch_pdl(kernel, dim3((unsigned)blocks), kQuantThreads, 0, s, reinterpret_cast<const T *>(in), rows, cols, row_stride,
-                                tiles, data, scales));
+    const bool whole = aligned(in, 16) && (row_stride * sizeof(T)) % 16 == 0 && cols % 8 == 0;
+    auto kernel = whole ? mx_quantize_kernel<T, false> : mx_quantize_kernel<T, true>;
+    GLOWB200_CUDA_OK(launch_pdl(kernel, dim3((unsigned)blocks), kThreads, 0, s, reinterpret_cast<const T *>(in), rows, cols, row_stride,
+                                (unsigned)tiles, data, scales));
     return GLOWB200_OK;
   });
 }
@@ -122,13 +206,13 @@ extern "C" int glowb200_microscaled_fp4_dequantize(const uint8_t *data, const ui
   GLOWB200_REQUIRE(data && scales && out, "NULL tensor pointer");
   GLOWB200_REQUIRE(aligned(data, 16) && aligned(scales, 16), "data and scales must start on 16-byte boundaries");
   GLOWB200_REQUIRE(aligned(out, float_type_bytes(out_type)), "the result is not aligned to its elements");
-  const int64_t chunks = rows * ((cols + 7) / 8), most = (int64_t)sm_count() * 32, blocks = (chunks + 255) / 256;
+  const int64_t tiles = mx_tiles(cols), blocks = mx_row_tiles(rows) * tiles;
+  GLOWB200_REQUIRE(blocks < (1ll << 31), "the matrix has more than 2^31 tiles of 128 x 128");
   return with_float_type(out_type, [&](auto *t) {
     using T = std::remove_pointer_t<decltype(t)>;
-    const bool vec = aligned(out, 16) && cols % 8 == 0;
-    auto kernel = vec ? mx_dequantize_kernel<T, true> : mx_dequantize_kernel<T, false>;
-    GLOWB200_CUDA_OK(launch_pdl(kernel, dim3((unsigned)(blocks < most ? blocks : most)), 256, 0, reinterpret_cast<cudaStream_t>(stream), data,
-                                scales, rows, cols, mx_tiles(cols), reinterpret_cast<T *>(out)));
+    auto kernel = aligned(out, 16) && cols % 8 == 0 ? mx_dequantize_kernel<T, false> : mx_dequantize_kernel<T, true>;
+    GLOWB200_CUDA_OK(launch_pdl(kernel, dim3((unsigned)blocks), kThreads, 0, reinterpret_cast<cudaStream_t>(stream), data, scales, rows, cols,
+                                (unsigned)tiles, reinterpret_cast<T *>(out)));
     return GLOWB200_OK;
   });
 }
