@@ -412,12 +412,13 @@ FcParams fc_params(void *out, const float *bias, int64_t M, int64_t K, int64_t N
 }
 
 int run_fc(void *out, int out_type, const void *a, const void *sa, const void *b, const void *sb, const float *bias, int64_t M, int64_t K,
-           int64_t N, int flags, int32_t *status, cudaStream_t s) {
+           int64_t N, int flags, int32_t *status, bool quantized, cudaStream_t s) {
   // The other kernel's time grows with the rows, which it adds up over a cluster, and shrinks with its splits of the depth: 64 rows
   // of 4096 x 4096 (K 1024, N 1024) 7.3 us (4.7) there and 7.1 (3.7) here, 32 rows 6.0 (4.1), 16 rows 5.2 (3.7), 64 rows of K
-  // 16384, N 2048 8.7 and 18.4, 128 rows of it 16.4.
+  // 16384, N 2048 8.7 and 18.4, 128 rows of it 16.4.  Behind a quantizing launch its clusters find their places late: 33 rows
+  // of 4096 x 4096 12.6 us with the launch, 9.3 here, of K 16384, N 2048 11.0 and 20.
   const int64_t k_blocks = (K + 255) / 256;
-  if (M <= 16 || (M <= 64 && k_blocks >= 8) || (M <= kFewRows && k_blocks >= 32))
+  if ((M <= 16 && !quantized) || (M <= 64 && k_blocks >= 8 && !quantized) || (M <= kFewRows && k_blocks >= 32))
     return run_fp4_few_rows(fc_params(out, bias, M, K, N, flags, status), out_type, a, sa, -1, 0, b, sb, K, s);
   const FcParams p = fc_params(out, bias, M, K, N, flags, status);
   return with_float_type(out_type, [&](auto *t) {
@@ -437,7 +438,8 @@ extern "C" int glowb200_microscaled_fp4_fc(void *out, int out_type, const uint8_
   if (M == 0 || N == 0) return GLOWB200_OK;
   GLOWB200_REQUIRE(in_scales, "NULL tensor pointer");
   GLOWB200_REQUIRE(aligned(in, 16) && aligned(in_scales, 16), "data and scales must start on 16-byte boundaries");
-  return run_fc(out, out_type, in, in_scales, weights, weights_scales, bias, M, K, N, flags, status, reinterpret_cast<cudaStream_t>(stream));
+  return run_fc(out, out_type, in, in_scales, weights, weights_scales, bias, M, K, N, flags, status, false,
+                reinterpret_cast<cudaStream_t>(stream));
 }
 
 extern "C" size_t glowb200_dynamic_microscaled_fp4_fc_workspace_bytes(int64_t M, int64_t K, int64_t N) {
@@ -458,11 +460,13 @@ extern "C" int glowb200_dynamic_microscaled_fp4_fc(void *out, int out_type, cons
   if (workspace == nullptr || workspace_bytes < need)
     return set_error(GLOWB200_ERR_WORKSPACE_TOO_SMALL, "workspace of %zu bytes given, %zu needed", workspace_bytes, need);
   GLOWB200_REQUIRE(aligned(workspace, 256), "workspace must be 256-byte aligned");
-  if (M <= kFewQuantizedRows)
+  // Every tile of 128 columns quantizes all rows for itself: 8 rows of N 16384 8.6 us, in two launches 10; 16 rows 12.5 and
+  // 10.4; 32 rows of N 4096 9.2 and 9.2.
+  if (M <= kFewQuantizedRows && M * ((N + 127) / 128) <= 1024)
     return run_fp4_few_rows(fc_params(out, bias, M, K, N, flags, status), out_type, in, nullptr, in_type, row_stride, weights, weights_scales, K,
                             reinterpret_cast<cudaStream_t>(stream));
   uint8_t *data = reinterpret_cast<uint8_t *>(workspace), *scales = data + align_up((size_t)(M * mx_pitch(K)), 256);
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   if (int rc = run_mx_quantize(in, in_type, M, K, row_stride, data, scales, s)) return rc;
-  return run_fc(out, out_type, data, scales, weights, weights_scales, bias, M, K, N, flags, status, s);
+  return run_fc(out, out_type, data, scales, weights, weights_scales, bias, M, K, N, flags, status, true, s);
 }
