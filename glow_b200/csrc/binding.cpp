@@ -708,11 +708,14 @@ PyObject *group_norm(PyObject *const *a) {
   if (!quant && !(FLOATS >> (int)type & 1)) bad_argument("out", a[10], FLOATS);
   const float *gamma = floats(a[2], "gamma", channels, x), *beta = floats(a[3], "beta", channels, x);
   const Tensor out = given_or_new(a[10], x.sizes(), type, x, "out");
-  const Workspace room(a[11], fn.glowb200_group_norm_workspace_bytes(images, pixels, channels, groups), x);
-  beside(room.t, "workspace", x);
+  const size_t need = fn.glowb200_group_norm_workspace_bytes(images, pixels, channels, groups);
+  Tensor room;  // (small images need none)
+  if (a[11] != Py_None) room = beside(cuda_tensor(a[11], "workspace", U8), "workspace", x);
+  else if (need > 0) room = empty({(int64_t)need}, at::kByte, x);
   invoke(fn.glowb200_group_norm, quant ? nullptr : out.data_ptr(), quant ? 0 : float_type(type), quant ? (int8_t *)out.data_ptr() : nullptr,
          real(a[7]), (int32_t)integer(a[8]), x.data_ptr(), float_type(x.scalar_type()), gamma, beta, images, pixels, channels, groups,
-         real(a[4]), (int)integer(a[5]), room.data(), room.bytes(), status_word(a[12], x), stream());
+         real(a[4]), (int)integer(a[5]), room.defined() ? room.data_ptr() : nullptr, room.defined() ? (size_t)room.numel() : 0,
+         status_word(a[12], x), stream());
   return a[10] == Py_None ? give(out) : same(a[10]);
 }
 

@@ -157,11 +157,18 @@ __device__ __forceinline__ void activate(float (&y)[N], int act) {
 #pragma unroll
     for (int k = 0; k < N; k++) asm("max.NaN.f32 %0, %0, %1;" : "+f"(y[k]) : "f"(0.0f));
   } else if (act == GLOWB200_NORM_ACT_SWISH) {
-    // (16-bit results: the fast exponential and quotient are off by some 2^-21)
+    if constexpr (sizeof(Out) == 2) {
+      // (16-bit results: the approximate exponential and reciprocal are off by some 2^-21)
 #pragma unroll
-    for (int k = 0; k < N; k++) {
-      if constexpr (sizeof(Out) == 2) y[k] = __fdividef(y[k], 1.0f + __expf(-y[k]));
-      else y[k] = y[k] / (1.0f + expf(-y[k]));
+      for (int k = 0; k < N; k++) {
+        float e;
+        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(y[k] * -1.4426950408889634f));
+        asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(1.0f + e));
+        y[k] *= e;
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < N; k++) y[k] = y[k] / (1.0f + expf(-y[k]));
     }
   }
 }
@@ -802,20 +809,31 @@ int launch_width(const NormParams &p, int vec, int64_t slice, cudaStream_t s) {
   else return vec == 8 ? launch_vec<T, 8, Out>(p, slice, s) : launch_vec<T, 2, Out>(p, slice, s);
 }
 
+// Blocks of the one launch's clusters: as few as hold a slice's pixels, eight at most; 0: they do not.
+int64_t single_blocks(int64_t slice, int vec, int64_t pixels) {
+  if (slice <= 0) return 0;
+  const int64_t most = (int64_t)rows_for(slice / vec, pixels) * (kHeld - 1);
+  for (int64_t blocks = 1; blocks <= 8; blocks *= 2)
+    if (blocks * most >= pixels) return blocks;
+  return 0;
+}
+// Whether every type and alignment of such an input takes the one launch, which needs no workspace.
+bool always_single(int64_t pixels, int64_t channels, int64_t groups) {
+  for (int bytes : {2, 4})
+    for (int vec : {16 / bytes, 4 / bytes, 1})
+      if (channels % vec == 0 && single_blocks(pick_slice(channels, groups, vec, bytes), vec, pixels) == 0) return false;
+  return true;
+}
+
 template <typename T, typename Out>
 int launch(NormParams p, cudaStream_t s) {
   const void *out = sizeof(Out) == 1 ? static_cast<const void *>(p.out_i8) : p.out;
   const int vec = side_by_side(p.in, out, sizeof(T), sizeof(Out), p.channels);
-  int64_t slice = pick_slice(p.channels, p.groups, vec, sizeof(T));
-  if (slice > 0) {  // ... over as few blocks as hold its pixels, eight at most
-    const int64_t rows = rows_for(slice / vec, p.pixels), most = rows * (kHeld - 1);
-    int64_t blocks = 1;
-    while (blocks < 8 && blocks * most < p.pixels) blocks *= 2;
-    if (blocks * most >= p.pixels) {
-      p.chunks = (int)blocks;
-      p.chunk_pixels = (p.pixels + blocks - 1) / blocks;
-      return launch_width<T, Out>(p, vec, slice, s);
-    }
+  const int64_t slice = pick_slice(p.channels, p.groups, vec, sizeof(T)), blocks_of_slice = single_blocks(slice, vec, p.pixels);
+  if (blocks_of_slice > 0) {
+    p.chunks = (int)blocks_of_slice;
+    p.chunk_pixels = (p.pixels + blocks_of_slice - 1) / blocks_of_slice;
+    return launch_width<T, Out>(p, vec, slice, s);
   }
   if (p.channels / vec <= kNormThreads) {
     const int64_t chunks = image_chunks(p.images, p.pixels, p.channels);
@@ -840,7 +858,7 @@ using namespace glowb200;
 
 extern "C" size_t glowb200_group_norm_workspace_bytes(int64_t images, int64_t pixels, int64_t channels, int64_t groups) {
   if (images <= 0 || pixels <= 0 || channels <= 0 || groups <= 0) return 0;
-  if (channels % groups != 0) return 0;
+  if (channels % groups != 0 || always_single(pixels, channels, groups)) return 0;
   const int64_t a = any_chunks(images, pixels, channels, groups), b = image_chunks(images, pixels, channels);
   return align_up((size_t)(images * groups) * 8, 256) + (size_t)(images * groups * (a > b ? a : b)) * 8;
 }
@@ -861,7 +879,7 @@ extern "C" int glowb200_group_norm(void *out, int out_type, int8_t *out_i8, floa
   GLOWB200_REQUIRE(aligned(in, float_type_bytes(in_type)) && (out_i8 != nullptr || aligned(out, float_type_bytes(out_type))),
                    "a tensor is not aligned to its elements");
   const size_t need = glowb200_group_norm_workspace_bytes(images, pixels, channels, groups);
-  if (workspace == nullptr || workspace_bytes < need)
+  if (need > 0 && (workspace == nullptr || workspace_bytes < need))
     return set_error(GLOWB200_ERR_WORKSPACE_TOO_SMALL, "workspace of %zu bytes given, %zu needed", workspace_bytes, need);
   GLOWB200_REQUIRE(aligned(workspace, 256), "workspace must be 256-byte aligned");
   NormParams p{};

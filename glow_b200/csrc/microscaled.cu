@@ -42,14 +42,17 @@ __global__ void __launch_bounds__(kThreads) mx_quantize_kernel(const T *__restri
   const int64_t pitch = 16 * ((cols + 31) / 32);
   const T *x = in + (at.row0 + at.first) * row_stride + at.col;
   const int64_t left = cols - at.col;
+  // (row r = 16 i + first of the block: r % 32 and r / 32 of its place in the scale tile are i's alone but for `first`)
+  uint8_t *out = data + (at.row0 + at.first) * pitch + at.col / 2, *out_scale = tile + at.first * 16 + ((lane & 15) >> 2);
+  const int mine = at.col / 2 < pitch ? at.rows - at.first : 0;  // (pitch: whole blocks)
   auto finish = [&](int i, const Eight<true, T> &v) {
-    const int r = i * 16 + at.first;
     uint32_t byte;
     const uint32_t codes = mx_block(v, byte);
-    if (r < at.rows && at.col / 2 < pitch) {  // (pitch: whole blocks)
-      *reinterpret_cast<uint32_t *>(data + (at.row0 + r) * pitch + at.col / 2) = codes;
-      if ((lane & 3) == 0) tile[(r & 31) * 16 + (r >> 5) * 4 + ((lane & 15) >> 2)] = (uint8_t)byte;
+    if (i * 16 < mine) {
+      *reinterpret_cast<uint32_t *>(out) = codes;
+      if ((lane & 3) == 0) out_scale[(i & 1) * 256 + (i >> 1) * 4] = (uint8_t)byte;
     }
+    out += 16 * pitch;
   };
   constexpr int kAtOnce = sizeof(T) == 4 ? 4 : 8;
 #pragma unroll
@@ -117,7 +120,7 @@ __global__ void __launch_bounds__(kThreads) mx_dequantize_kernel(const uint8_t *
   for (int i = 0; i < 8; i++) {
     if (i * 16 >= at.rows) break;
     const int r = i * 16 + at.first;
-    const float scale = mx_scale(tile[(r & 31) * 16 + (r >> 5) * 4 + ((lane & 15) >> 2)]);
+    const float scale = mx_scale(tile[at.first * 16 + ((lane & 15) >> 2) + (i & 1) * 256 + (i >> 1) * 4]);
     float v[8];
 #pragma unroll
     for (int k = 0; k < 4; k++) {

@@ -2,6 +2,8 @@
 #pragma once
 #include <cuda_bf16.h>
 
+#include <type_traits>
+
 #include "common.cuh"
 
 namespace glowb200 {
@@ -100,12 +102,23 @@ struct Eight {
 // scale byte.  Infinities and NaNs: byte 255, codes 0.
 template <bool VEC, typename T>
 __device__ __forceinline__ uint32_t mx_block(const Eight<VEC, T> &x, uint32_t &byte) {
+  uint32_t top = 0;  // the largest magnitude's bits
   float v[8];
+  if constexpr (sizeof(T) == 4) {
 #pragma unroll
-  for (int k = 0; k < 8; k++) v[k] = to_float(x.w[k]);
-  uint32_t top = 0;
+    for (int k = 0; k < 8; k++) {
+      v[k] = x.w[k];
+      top = max(top, __float_as_uint(v[k]) & 0x7FFFFFFFu);
+    }
+  } else {  // two at a time: magnitudes are ordered as their bits are
+    const uint32_t *w = reinterpret_cast<const uint32_t *>(x.w);
+    uint32_t most = __vmaxu2(__vmaxu2(w[0] & 0x7FFF7FFFu, w[1] & 0x7FFF7FFFu), __vmaxu2(w[2] & 0x7FFF7FFFu, w[3] & 0x7FFF7FFFu));
+    most = max(most & 0xFFFFu, most >> 16);
+    if constexpr (std::is_same_v<T, __half>) top = __float_as_uint(__half2float(__ushort_as_half((unsigned short)most)));
+    else top = most << 16;
 #pragma unroll
-  for (int k = 0; k < 8; k++) top = max(top, __float_as_uint(v[k]) & 0x7FFFFFFFu);
+    for (int k = 0; k < 8; k++) v[k] = to_float(x.w[k]);
+  }
   top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
   top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
   byte = mx_scale_byte(top);

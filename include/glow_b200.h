@@ -690,7 +690,8 @@ int glowb200_dynamic_microscaled_fp4_fc(void *out, int out_type, const void *in,
  *   y = act((x - mean) / sqrt(variance + eps) * gamma[c] + beta[c])
  * gamma, beta: fp32 [channels] or NULL (1 and 0).  The result, dense like `in`, is rounded once to out_type, or to int8
  * as glowb200_element_quantize_i8 does it with quant_scale / quant_offset: exactly one of out and out_i8 is given.
- * act: GLOWB200_NORM_ACT_*.  The workspace (256-byte aligned) must hold glowb200_group_norm_workspace_bytes(...). */
+ * act: GLOWB200_NORM_ACT_*.  `out` may be `in`.  The workspace (256-byte aligned) must hold
+ * glowb200_group_norm_workspace_bytes(...) bytes; small images need none. */
 #define GLOWB200_NORM_ACT_NONE 0
 #define GLOWB200_NORM_ACT_RELU 1
 #define GLOWB200_NORM_ACT_SWISH 2 /* y / (1 + exp(-y)) */

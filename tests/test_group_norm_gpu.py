@@ -108,6 +108,12 @@ def test_int8_result_is_the_quantize_node_behind_it(shape, G, dtype):
 
 
 def test_given_result_workspace_and_refusals():
+    x, gamma, beta = case(14, (1, 300, 300, 64), "fp16")
+    need = int(_lib.lib().glowb200_group_norm_workspace_bytes(1, 90000, 64, 8))
+    room = torch.full((need,), 0xFF, dtype=torch.uint8, device=DEV)
+    assert torch.equal(ops.group_norm(x, 8, gamma, beta, workspace=room), ops.group_norm(x, 8, gamma, beta))
+    with pytest.raises(_lib.GlowB200Error, match="workspace"):
+        ops.group_norm(x, 8, gamma, beta, workspace=room[:need - 1])
     x, gamma, beta = case(13, (2, 8, 8, 32), "fp16")
     need = int(_lib.lib().glowb200_group_norm_workspace_bytes(2, 64, 32, 4))
     room = torch.full((max(need, 8),), 0xFF, dtype=torch.uint8, device=DEV)

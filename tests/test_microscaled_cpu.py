@@ -23,7 +23,7 @@ def test_sizes(l):
     assert l.glowb200_microscaled_fp4_scales_bytes(0, 64) == 0 and l.glowb200_microscaled_fp4_scales_bytes(-1, 64) == 0
     assert l.glowb200_dynamic_microscaled_fp4_fc_workspace_bytes(5, 100, 7) >= 5 * 64 + 512
     assert l.glowb200_dynamic_microscaled_fp4_fc_workspace_bytes(-5, 100, 7) == 0
-    assert l.glowb200_group_norm_workspace_bytes(0, 9, 8, 2) == 0
+    assert l.glowb200_group_norm_workspace_bytes(0, 9, 8, 2) == 0 and l.glowb200_group_norm_workspace_bytes(3, 1 << 20, 64, 8) > 0
 
 
 @pytest.mark.parametrize("args", [(FAKE, 3, 4, 64, 64, FAKE, FAKE), (FAKE, 0, -1, 64, 64, FAKE, FAKE), (FAKE, 0, 4, 0, 64, FAKE, FAKE),
@@ -63,7 +63,8 @@ def test_dynamic_fc_refuses(l):
 @pytest.mark.parametrize("change,code", [(dict(groups=3), 1), (dict(groups=0), 1), (dict(channels=0), 1), (dict(images=-1), 1), (dict(act=3), 1),
                                          (dict(eps=-1.0), 1), (dict(eps=float("nan")), 1), (dict(in_type=4), 1), (dict(out_type=4), 1),
                                          (dict(out_i8=FAKE), 1), (dict(out=None), 1), (dict(inp=None), 1), (dict(inp=C.c_void_p(4097)), 1),
-                                         (dict(ws=None), 3), (dict(size=7), 3), (dict(ws=C.c_void_p(4096 + 64)), 1)])
+                                         (dict(pixels=1 << 20, ws=None), 3), (dict(pixels=1 << 20, size=7), 3),
+                                         (dict(pixels=1 << 20, ws=C.c_void_p(4096 + 64)), 1)])
 def test_group_norm_refuses(l, change, code):
     v = dict(out=FAKE, out_type=0, out_i8=None, scale=1.0, offset=0, inp=FAKE, in_type=1, gamma=None, beta=None, images=2, pixels=9, channels=8,
              groups=2, eps=1e-5, act=0, ws=FAKE, size=1 << 20)
