@@ -397,7 +397,8 @@ int launch(const void *a, const void *sa, const void *b, const void *sb, int64_t
 }
 
 int check_fc(const void *out, int out_type, const void *in, const void *weights, const void *weights_scales, int64_t M, int64_t K, int64_t N, int flags) {
-  GLOWB200_REQUIRE(M >= 0 && N >= 0 && K > 0 && M < (1ll << 31) && N < (1ll << 31) && K < (1ll << 31), "matrix dimensions out of range");
+  constexpr int64_t kMost = (1ll << 31) - 1024;  // (tiles reach beyond the last row and column)
+  GLOWB200_REQUIRE(M >= 0 && N >= 0 && K > 0 && M <= kMost && N <= kMost && K <= kMost, "matrix dimensions out of range");
   GLOWB200_REQUIRE(out_type >= 0 && out_type <= 2, "float type %d is not GLOWB200_FLOAT32, _FLOAT16 or _BFLOAT16", out_type);
   GLOWB200_REQUIRE((flags & ~GLOWB200_FC_FUSE_RELU) == 0, "flags other than GLOWB200_FC_FUSE_RELU");
   if (M == 0 || N == 0) return GLOWB200_OK;

@@ -19,6 +19,7 @@ namespace glowb200 {
 namespace {
 
 constexpr int kNormThreads = 512;
+constexpr int kMostShared = 232448;  // bytes that a block can have: what kernels are allowed, whatever a launch takes (calls may overlap)
 
 struct NormParams {
   const void *in;
@@ -772,7 +773,7 @@ int launch_unit(NormParams p, int64_t slice, cudaStream_t s) {
     const int64_t each = (p.chunk_pixels + p.rows - 1) / p.rows;
     const size_t shared = Held<T, VEC>::kCan ? p.held_at + Held<T, VEC>::bytes((int)threads, (int)align_up((size_t)each, 4)) : own;
     auto kernel = norm_single_kernel<T, VEC, UNIT, Out>;
-    GLOWB200_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)shared));
+    GLOWB200_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostShared));
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(p.images * p.slices * p.chunks));
     cfg.blockDim = dim3(threads);
@@ -790,7 +791,7 @@ int launch_unit(NormParams p, int64_t slice, cudaStream_t s) {
     return GLOWB200_OK;
   }
   auto run = [&](auto kernel, size_t shared) {
-    GLOWB200_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)shared));
+    GLOWB200_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostShared));
     GLOWB200_CUDA_OK(launch_pdl(kernel, dim3((unsigned)(p.images * p.chunks)), threads, shared, s, p));
     return GLOWB200_OK;
   };

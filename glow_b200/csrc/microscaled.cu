@@ -25,14 +25,38 @@ struct TilePlace {
   }
 };
 
-// RAGGED: rows off 16-byte boundaries, or whose last eight columns are not all there.  Their elements come one to a lane, 32
-// neighbours at a time, and change places in shared memory: eight single loads to a lane would ask for eight times as
-// many lines.
-template <typename T, bool RAGGED>
+// Rows off 16-byte boundaries, or whose last eight columns are not all there, come in words W of four bytes or two, one to a
+// lane, neighbours to neighbouring lanes, and change places in shared memory: loads of a lane's own eight elements would ask
+// for as many lines eight times.  (W void: whole rows, 16 bytes to a lane.)
+template <typename T, typename W>
+struct Words {
+  static constexpr int kRow = 128 * sizeof(T) / sizeof(W) / 32, kBoth = 2 * kRow;  // words of a lane: of a row, of the warp's two
+  static constexpr int kElements = sizeof(W) / sizeof(T) > 0 ? sizeof(W) / sizeof(T) : 1;
+  bool in[kRow];       // the word's column is there
+  int rows;            // of the block from the warp's first row on
+  __device__ __forceinline__ Words(const TilePlace &at, int64_t cols) {
+    const int64_t first = at.col - (threadIdx.x & 15) * 8;
+#pragma unroll
+    for (int k = 0; k < kRow; k++) in[k] = first + (k * 32 + (int)(threadIdx.x & 31)) * kElements < cols;
+    rows = at.rows - (at.first & ~1);
+  }
+  // the lane's first word of the warp's first row
+  template <typename P>
+  static __device__ __forceinline__ P *start(P *base, const TilePlace &at, int64_t stride) {
+    return base + (at.row0 + (at.first & ~1)) * stride + at.col - (threadIdx.x & 15) * 8 + (threadIdx.x & 31) * kElements;
+  }
+};
+template <typename T>
+struct Words<T, void> {
+  static constexpr int kBoth = 1;
+};
+
+template <typename T, typename W>
 __global__ void __launch_bounds__(kThreads) mx_quantize_kernel(const T *__restrict__ in, int64_t rows, int64_t cols, int64_t row_stride,
                                                                unsigned tiles, uint8_t *__restrict__ data, uint8_t *__restrict__ scales) {
+  constexpr bool kWhole = std::is_void_v<W>;
   __shared__ __align__(16) uint8_t tile[512];
-  __shared__ __align__(16) T staged[RAGGED ? kThreads * 8 : 8];
+  __shared__ __align__(16) T staged[kWhole ? 8 : kThreads * 8];
   pdl_wait();
   pdl_launch_dependents();
   const TilePlace at(rows, tiles);
@@ -40,8 +64,6 @@ __global__ void __launch_bounds__(kThreads) mx_quantize_kernel(const T *__restri
   if (threadIdx.x < 32) reinterpret_cast<uint4 *>(tile)[threadIdx.x] = make_uint4(0, 0, 0, 0);
   __syncthreads();
   const int64_t pitch = 16 * ((cols + 31) / 32);
-  const T *x = in + (at.row0 + at.first) * row_stride + at.col;
-  const int64_t left = cols - at.col;
   // (row r = 16 i + first of the block: r % 32 and r / 32 of its place in the scale tile are i's alone but for `first`)
   uint8_t *out = data + (at.row0 + at.first) * pitch + at.col / 2, *out_scale = tile + at.first * 16 + ((lane & 15) >> 2);
   const int mine = at.col / 2 < pitch ? at.rows - at.first : 0;  // (pitch: whole blocks)
@@ -55,41 +77,49 @@ __global__ void __launch_bounds__(kThreads) mx_quantize_kernel(const T *__restri
     out += 16 * pitch;
   };
   constexpr int kAtOnce = sizeof(T) == 4 ? 4 : 8;
+  if constexpr (kWhole) {
+    const T *x = in + (at.row0 + at.first) * row_stride + at.col;
+    const int64_t left = cols - at.col;
 #pragma unroll
-  for (int i0 = 0; i0 < 8; i0 += kAtOnce) {
-    if (i0 * 16 >= at.rows) break;
-    Eight<true, T> v[kAtOnce];
-    if constexpr (!RAGGED) {
+    for (int i0 = 0; i0 < 8; i0 += kAtOnce) {
+      if (i0 * 16 >= at.rows) break;
+      Eight<true, T> v[kAtOnce];
 #pragma unroll
       for (int i = 0; i < kAtOnce; i++) v[i].load(x + (int64_t)(i0 + i) * 16 * row_stride, (i0 + i) * 16 + at.first < at.rows ? left : 0);
 #pragma unroll
       for (int i = 0; i < kAtOnce; i++)
         if ((i0 + i) * 16 < at.rows) finish(i0 + i, v[i]);
-    } else {
-      // the warp's two rows of 128 columns, 32 at a time: element e of them is row e / 128, column e % 128
-      T *mine = staged + (threadIdx.x & ~31) * 8;
-      const int64_t col0 = at.col - (lane & 15) * 8;
-      const int row = (at.first & ~1);
-      T w[kAtOnce][8];
+    }
+  } else {
+    using S = Words<T, W>;
+    const S words(at, cols);
+    const T *x = S::start(in, at, row_stride);
+    W *mine_here = reinterpret_cast<W *>(staged + (threadIdx.x & ~31) * 8);
 #pragma unroll
-      for (int i = 0; i < kAtOnce; i++)
+    for (int i0 = 0; i0 < 8; i0 += kAtOnce) {
+      if (i0 * 16 >= at.rows) break;
+      W w[kAtOnce][S::kBoth];
 #pragma unroll
-        for (int k = 0; k < 8; k++) {
-          const int r = (i0 + i) * 16 + row + (k >> 2);
-          const int64_t c = col0 + (k & 3) * 32 + lane;
-          w[i][k] = r < at.rows && c < cols ? in[(at.row0 + r) * row_stride + c] : from_float<T>(0.0f);
-        }
+      for (int i = 0; i < kAtOnce; i++) {
+#pragma unroll
+        for (int k = 0; k < S::kBoth; k++)
+          w[i][k] = words.in[k % S::kRow] && (i0 + i) * 16 + k / S::kRow < words.rows
+                        ? __ldg(reinterpret_cast<const W *>(x + (k / S::kRow) * row_stride + (k % S::kRow) * 32 * S::kElements))
+                        : W(0);
+        x += 16 * row_stride;
+      }
 #pragma unroll
       for (int i = 0; i < kAtOnce; i++)
         if ((i0 + i) * 16 < at.rows) {
           __syncwarp();
 #pragma unroll
-          for (int k = 0; k < 8; k++) mine[k * 32 + lane] = w[i][k];
+          for (int k = 0; k < S::kBoth; k++) mine_here[k * 32 + lane] = w[i][k];
           __syncwarp();
+          Eight<true, T> v;
 #pragma unroll
           for (int k = 0; k < (int)(8 * sizeof(T) / 16); k++)
-            reinterpret_cast<uint4 *>(v[i].w)[k] = reinterpret_cast<const uint4 *>(mine + lane * 8)[k];
-          finish(i0 + i, v[i]);
+            reinterpret_cast<uint4 *>(v.w)[k] = reinterpret_cast<const uint4 *>(staged + threadIdx.x * 8)[k];
+          finish(i0 + i, v);
         }
     }
   }
@@ -98,11 +128,12 @@ __global__ void __launch_bounds__(kThreads) mx_quantize_kernel(const T *__restri
     reinterpret_cast<uint4 *>(scales + (size_t)blockIdx.x * 512)[threadIdx.x] = reinterpret_cast<const uint4 *>(tile)[threadIdx.x];
 }
 
-template <typename T, bool RAGGED>
+template <typename T, typename W>
 __global__ void __launch_bounds__(kThreads) mx_dequantize_kernel(const uint8_t *__restrict__ data, const uint8_t *__restrict__ scales, int64_t rows,
                                                                  int64_t cols, unsigned tiles, T *__restrict__ out) {
+  constexpr bool kWhole = std::is_void_v<W>;
   __shared__ __align__(16) uint8_t tile[512];
-  __shared__ __align__(16) T staged[RAGGED ? kThreads * 8 : 8];
+  __shared__ __align__(16) T staged[kWhole ? 8 : kThreads * 8];
   pdl_wait();
   pdl_launch_dependents();
   const TilePlace at(rows, tiles);
@@ -116,11 +147,9 @@ __global__ void __launch_bounds__(kThreads) mx_dequantize_kernel(const uint8_t *
   if (threadIdx.x < 32)
     reinterpret_cast<uint4 *>(tile)[threadIdx.x] = __ldg(reinterpret_cast<const uint4 *>(scales + (size_t)blockIdx.x * 512) + threadIdx.x);
   __syncthreads();
-#pragma unroll
-  for (int i = 0; i < 8; i++) {
-    if (i * 16 >= at.rows) break;
-    const int r = i * 16 + at.first;
-    const float scale = mx_scale(tile[at.first * 16 + ((lane & 15) >> 2) + (i & 1) * 256 + (i >> 1) * 4]);
+  const uint8_t *my_scale = tile + at.first * 16 + ((lane & 15) >> 2);
+  auto numbers = [&](int i, uint32_t (&w)[2 * sizeof(T)]) {
+    const float scale = mx_scale(my_scale[(i & 1) * 256 + (i >> 1) * 4]);
     float v[8];
 #pragma unroll
     for (int k = 0; k < 4; k++) {
@@ -128,35 +157,56 @@ __global__ void __launch_bounds__(kThreads) mx_dequantize_kernel(const uint8_t *
       v[2 * k] = n.x * scale;
       v[2 * k + 1] = n.y * scale;
     }
-    uint32_t w[2 * sizeof(T)];
 #pragma unroll
     for (int k = 0; k < (int)(2 * sizeof(T)); k++) {
       if constexpr (sizeof(T) == 4) w[k] = __float_as_uint(v[k]);
       else w[k] = pack2(v[2 * k], v[2 * k + 1], T());
     }
-    if constexpr (!RAGGED) {
-      if (r < at.rows && at.col < cols) {
-        T *o = out + (at.row0 + r) * cols + at.col;
+  };
+  auto put = [](T *to, const uint32_t (&w)[2 * sizeof(T)]) {
 #pragma unroll
-        for (int k = 0; k < (int)(sizeof(T) / 2); k++)
-          reinterpret_cast<uint4 *>(o)[k] = make_uint4(w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]);
-      }
-    } else {
-      T *mine = staged + (threadIdx.x & ~31) * 8;
+    for (int k = 0; k < (int)(sizeof(T) / 2); k++)
+      reinterpret_cast<uint4 *>(to)[k] = make_uint4(w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]);
+  };
+  uint32_t w[2 * sizeof(T)];
+  if constexpr (kWhole) {
+    T *o = out + (at.row0 + at.first) * cols + at.col;
+    const int mine = at.col < cols ? at.rows - at.first : 0;
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      if (i * 16 >= at.rows) break;
+      numbers(i, w);
+      if (i * 16 < mine) put(o, w);
+      o += 16 * cols;
+    }
+  } else {
+    using S = Words<T, W>;
+    const S words(at, cols);
+    T *o = S::start(out, at, cols);
+    const W *mine_here = reinterpret_cast<const W *>(staged + (threadIdx.x & ~31) * 8);
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      if (i * 16 >= at.rows) break;
+      numbers(i, w);
+      __syncwarp();
+      put(staged + threadIdx.x * 8, w);
       __syncwarp();
 #pragma unroll
-      for (int k = 0; k < (int)(sizeof(T) / 2); k++)
-        reinterpret_cast<uint4 *>(mine + lane * 8)[k] = make_uint4(w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]);
-      __syncwarp();
-      const int64_t col0 = at.col - (lane & 15) * 8;
-#pragma unroll
-      for (int k = 0; k < 8; k++) {
-        const int rr = i * 16 + (at.first & ~1) + (k >> 2);
-        const int64_t c = col0 + (k & 3) * 32 + lane;
-        if (rr < at.rows && c < cols) out[(at.row0 + rr) * cols + c] = mine[k * 32 + lane];
-      }
+      for (int k = 0; k < S::kBoth; k++)
+        if (words.in[k % S::kRow] && i * 16 + k / S::kRow < words.rows)
+          *reinterpret_cast<W *>(o + (k / S::kRow) * cols + (k % S::kRow) * 32 * S::kElements) = mine_here[k * 32 + lane];
+      o += 16 * cols;
     }
   }
+}
+
+// Calls f with a null pointer of the word that rows `stride` elements of T apart, `cols` of them there, are taken in.
+template <typename T, typename F>
+int with_word(const void *base, int64_t stride, int64_t cols, F f) {
+  if (aligned(base, 16) && stride * sizeof(T) % 16 == 0 && cols % 8 == 0) return f(static_cast<void *>(nullptr));
+  if constexpr (sizeof(T) == 2)
+    if (!aligned(base, 4) || stride % 2 != 0 || cols % 2 != 0) return f(static_cast<uint16_t *>(nullptr));
+  return f(static_cast<uint32_t *>(nullptr));
 }
 
 int check_matrix(int64_t rows, int64_t cols) {
@@ -172,11 +222,11 @@ int run_mx_quantize(const void *in, int in_type, int64_t rows, int64_t cols, int
   GLOWB200_REQUIRE(blocks < (1ll << 31), "the matrix has more than 2^31 tiles of 128 x 128");
   return with_float_type(in_type, [&](auto *t) {
     using T = std::remove_pointer_t<decltype(t)>;
-    const bool whole = aligned(in, 16) && (row_stride * sizeof(T)) % 16 == 0 && cols % 8 == 0;
-    auto kernel = whole ? mx_quantize_kernel<T, false> : mx_quantize_kernel<T, true>;
-    GLOWB200_CUDA_OK(launch_pdl(kernel, dim3((unsigned)blocks), kThreads, 0, s, reinterpret_cast<const T *>(in), rows, cols, row_stride,
-                                (unsigned)tiles, data, scales));
-    return GLOWB200_OK;
+    return with_word<T>(in, row_stride, cols, [&](auto *w) {
+      GLOWB200_CUDA_OK(launch_pdl(mx_quantize_kernel<T, std::remove_pointer_t<decltype(w)>>, dim3((unsigned)blocks), kThreads, 0, s,
+                                  reinterpret_cast<const T *>(in), rows, cols, row_stride, (unsigned)tiles, data, scales));
+      return GLOWB200_OK;
+    });
   });
 }
 
@@ -213,9 +263,10 @@ extern "C" int glowb200_microscaled_fp4_dequantize(const uint8_t *data, const ui
   GLOWB200_REQUIRE(blocks < (1ll << 31), "the matrix has more than 2^31 tiles of 128 x 128");
   return with_float_type(out_type, [&](auto *t) {
     using T = std::remove_pointer_t<decltype(t)>;
-    auto kernel = aligned(out, 16) && cols % 8 == 0 ? mx_dequantize_kernel<T, false> : mx_dequantize_kernel<T, true>;
-    GLOWB200_CUDA_OK(launch_pdl(kernel, dim3((unsigned)blocks), kThreads, 0, reinterpret_cast<cudaStream_t>(stream), data, scales, rows, cols,
-                                (unsigned)tiles, reinterpret_cast<T *>(out)));
-    return GLOWB200_OK;
+    return with_word<T>(out, cols, cols, [&](auto *w) {
+      GLOWB200_CUDA_OK(launch_pdl(mx_dequantize_kernel<T, std::remove_pointer_t<decltype(w)>>, dim3((unsigned)blocks), kThreads, 0,
+                                  reinterpret_cast<cudaStream_t>(stream), data, scales, rows, cols, (unsigned)tiles, reinterpret_cast<T *>(out)));
+      return GLOWB200_OK;
+    });
   });
 }

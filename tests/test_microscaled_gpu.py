@@ -221,6 +221,27 @@ def test_rows_of_one_product_do_not_depend_on_the_others():
     assert same(all_rows[0], all_rows[5])
 
 
+@pytest.mark.parametrize("M,N", [(4, 96), (300, 96), (300, 256)])
+def test_results_off_16_byte_boundaries(M, N):
+    """Into a view two bytes behind a boundary: the same bits, and nothing beside them."""
+    w, ws = ops.microscaled_fp4_quantize(rows_of(31, N, 320, "fp32").to(DEV))
+    x = rows_of(32, M, 320, "bf16").to(DEV)
+    whole = torch.full((M * N + 9,), 7.0, dtype=torch.bfloat16, device=DEV)
+    out = whole[1:1 + M * N].view(M, N)
+    assert ops.dynamic_microscaled_fp4_fc(x, w, ws, out=out) is out
+    assert same(out, ops.dynamic_microscaled_fp4_fc(x, w, ws)) and (whole[0] == 7) and (whole[1 + M * N:] == 7).all()
+
+
+@pytest.mark.parametrize("M", [1, 20, 129, 300])
+def test_nothing_is_written_beside_the_result(M):
+    """Rows and columns of a tile that are not the matrix's leave what lies behind it alone."""
+    w, ws = ops.microscaled_fp4_quantize(rows_of(33, 72, 96, "fp32").to(DEV))
+    a, sa = ops.microscaled_fp4_quantize(rows_of(34, M, 96, "fp32").to(DEV))
+    whole = torch.full((M * 72 + 4096,), 7.0, dtype=torch.float32, device=DEV)
+    ops.microscaled_fp4_fc(a, sa, w, ws, out=whole[:M * 72].view(M, 72))
+    assert (whole[M * 72:] == 7).all()
+
+
 def test_empty_results():
     w, ws = ops.microscaled_fp4_quantize(torch.randn(40, 64, device=DEV))
     assert ops.dynamic_microscaled_fp4_fc(torch.empty(0, 64, device=DEV), w, ws).shape == (0, 40)
