@@ -122,13 +122,11 @@ fp4_few_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
           tmem_copy_scales<false>(t_sa + 4 * h, smem_desc_rows16(sa_addr + 512 * h));
           tmem_copy_scales<false>(t_sb + 4 * h, smem_desc_rows16(sa_addr + 1024 + 512 * h));
         }
-        const int steps = min(4, p.fc.k_steps - 4 * kb);
 #pragma unroll
-        for (int k = 0; k < 4; k++) {
+        for (int k = 0; k < 4; k++) {  // (what lies behind the depth is zeros)
           const uint32_t id = (uint32_t)(k & 1) * 2;
-          if (k < steps)
-            umma_mxf4<false>(tmem_base, a_desc + (uint64_t)(k * (kUmmaK >> 4)), b_desc + (uint64_t)(k * (kUmmaK >> 4)),
-                             idesc_mxf4(kBlockM, NT) | id << 4 | id << 29, t_sa + 4 * (k >> 1), t_sb + 4 * (k >> 1), kb != first || k != 0);
+          umma_mxf4<false>(tmem_base, a_desc + (uint64_t)(k * (kUmmaK >> 4)), b_desc + (uint64_t)(k * (kUmmaK >> 4)),
+                           idesc_mxf4(kBlockM, NT) | id << 4 | id << 29, t_sa + 4 * (k >> 1), t_sb + 4 * (k >> 1), k != 0 ? 1u : (uint32_t)(kb != first));
         }
         if (kb + S::kStages < last) umma_commit(&empty[s]);  // (nobody waits for a stage that is not filled again)
         if (kb + 1 == last) umma_commit(acc_full);
@@ -142,11 +140,13 @@ fp4_few_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
       // each is a column of the product of its own, and nobody reads it.
       const In *in = reinterpret_cast<const In *>(p.in);
       constexpr int kBatch = sizeof(In) == 4 ? 2 : 4;  // rows of a warp on their way at once
-      const int items = (last - first) * p.fc.M;  // (k-block, row), dealt to the warps in turn
-      int block = 0, row = w;                     // of the warp's next item; block: counted from the first
+      // (k-block, row), dealt in turn to so many warps that none skips kStages blocks: a wait by parity is one for the phase
+      // before the present one at most, and a warp further ahead would find a stage empty that is two rounds behind.
+      const int items = (last - first) * p.fc.M, dealt = min(kWorkers, S::kStages * p.fc.M);
+      int block = 0, row = w;  // of the warp's next item; block: counted from the first
       for (; row >= p.fc.M; row -= p.fc.M) block++;
       bool live = true;
-      for (int i0 = w; i0 < items && live; i0 += kBatch * kWorkers) {
+      for (int i0 = w < dealt ? w : items; i0 < items && live; i0 += kBatch * dealt) {
         Eight<VEC, In> x[kBatch];
         int blocks[kBatch], rows[kBatch];
 #pragma unroll
@@ -154,12 +154,12 @@ fp4_few_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
           blocks[i] = block;
           rows[i] = row;
           const int64_t col = (int64_t)(first + block) * 256 + lane * 8;
-          x[i].load(in + (int64_t)row * p.row_stride + col, i0 + i * kWorkers < items ? p.cols - col : 0);
-          for (row += kWorkers; row >= p.fc.M; row -= p.fc.M) block++;
+          x[i].load(in + (int64_t)row * p.row_stride + col, i0 + i * dealt < items ? p.cols - col : 0);
+          for (row += dealt; row >= p.fc.M; row -= p.fc.M) block++;
         }
 #pragma unroll
         for (int i = 0; i < kBatch; i++) {
-          if (i0 + i * kWorkers >= items || !live) break;
+          if (i0 + i * dealt >= items || !live) break;
           const int s = blocks[i] % S::kStages, r = rows[i];
           if (!warp_wait(&empty[s], (uint32_t)(blocks[i] / S::kStages & 1) ^ 1, abort_flag)) { live = false; break; }
           uint32_t byte;
@@ -289,8 +289,14 @@ int run_fp4_few_rows(const FcParams &fc, int out_type, const void *in, const voi
                      const void *weights, const void *weights_scales, int64_t K, cudaStream_t s) {
   FewRowsParams p{fc, in, row_stride, K, 1, (fc.k_steps + 3) / 4};
   const int64_t tiles = (fc.N + kBlockM - 1) / kBlockM;
-  const int at_once = fc.M <= 64 ? 2 : 1;
-  while (p.splits < kMostSplits && tiles * p.splits * 2 <= at_once * kB200Sms && p.splits * 2 <= p.k_blocks) p.splits *= 2;
+  // Blocks for the SMs once: one token of 4096 x 4096 takes 6.4, 5.5, 4.7 and 5.0 us in 1, 2, 4 and 8 splits (32 to 256 blocks), of
+  // K 4096, N 16384 6.6 and 7.2 in 1 and 2, of 8192 x 8192 10.2, 7.5, 7.2 and 10.8.  Twice where a block has more than 32
+  // pieces of rows to quantize: 16 rows of 4096 x 4096 7.0 and 6.6, 8 of N 16384 9.3 and 8.2 (8 of N 4096 5.3 and 5.8).
+  auto fits = [&](int splits) {
+    const bool much = in_type >= 0 && fc.M * (p.k_blocks / (splits / 2)) > 32;
+    return splits <= kMostSplits && splits <= p.k_blocks && tiles * splits <= (much ? 2 : 1) * kB200Sms;
+  };
+  while (fits(p.splits * 2)) p.splits *= 2;
   CUtensorMap mw, msw;
   if (int rc = make_data_map(&mw, weights, fc.N, mx_pitch(K), kBlockM)) return rc;
   if (int rc = make_scale_map(&msw, weights_scales, mx_row_tiles(fc.N), mx_tiles(K), 1)) return rc;

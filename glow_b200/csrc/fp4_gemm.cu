@@ -174,6 +174,9 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
       const uint32_t d_tmem = tmem_base + (uint32_t)(buf * (BLOCK_N - S::kShared));
       // The scales of a stage have columns of their own: a stage that is full again was empty, so the MMAs that read them are done.
       bool ready = mbar_try_wait(&full[ring.at], ring.round);
+      // (Four MMAs whatever is left of the depth: what lies behind it is loaded as zeros under scales of 0.  Choosing among them
+      // and not unrolling cost a sixteenth of a block's time where few blocks run.)
+#pragma unroll 2
       for (int kb = 0; kb < k_blocks; kb++) {
         const int s = ring.at;
         if (!__all_sync(0xffffffffu, ready) && !warp_wait(&full[s], ring.round, abort_flag)) { live = false; break; }
@@ -192,14 +195,12 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
             for (int r = 0; r < S::kRowTiles; r++)
               tmem_copy_scales<PAIR>(t_sb + (uint32_t)(4 * (h * S::kRowTiles + r)), smem_desc_rows16(sb_addr + 1024 * r + 512 * h));
           }
-          const int steps = min(4, p.k_steps - 4 * kb);
 #pragma unroll
           for (int k = 0; k < 4; k++) {
             const uint32_t id = (uint32_t)(k & 1) * 2;  // which two of a scale word's four bytes
-            if (k < steps)
-              umma_mxf4<PAIR>(d_tmem, a_desc + (uint64_t)(k * (kUmmaK >> 4)), b_desc + (uint64_t)(k * (kUmmaK >> 4)),
-                        idesc_mxf4(S::kRows, BLOCK_N) | id << 4 | id << 29, t_sa + 4 * (k >> 1),
-                        t_sb + (uint32_t)(4 * S::kRowTiles * (k >> 1) + (half_tile >> 5)), (kb | k) != 0);
+            umma_mxf4<PAIR>(d_tmem, a_desc + (uint64_t)(k * (kUmmaK >> 4)), b_desc + (uint64_t)(k * (kUmmaK >> 4)),
+                            idesc_mxf4(S::kRows, BLOCK_N) | id << 4 | id << 29, t_sa + 4 * (k >> 1),
+                            t_sb + (uint32_t)(4 * S::kRowTiles * (k >> 1) + (half_tile >> 5)), k != 0 ? 1u : (uint32_t)(kb != 0));
           }
           if constexpr (PAIR) umma_commit_pair(&empty[s]);
           else umma_commit(&empty[s]);
@@ -415,11 +416,11 @@ FcParams fc_params(void *out, const float *bias, int64_t M, int64_t K, int64_t N
 int run_fc(void *out, int out_type, const void *a, const void *sa, const void *b, const void *sb, const float *bias, int64_t M, int64_t K,
            int64_t N, int flags, int32_t *status, bool quantized, cudaStream_t s) {
   // The other kernel's time grows with the rows, which it adds up over a cluster, and shrinks with its splits of the depth: 64 rows
-  // of 4096 x 4096 (K 1024, N 1024) 7.3 us (4.7) there and 7.1 (3.7) here, 32 rows 6.0 (4.1), 16 rows 5.2 (3.7), 64 rows of K
-  // 16384, N 2048 8.7 and 18.4, 128 rows of it 16.4.  Behind a quantizing launch its clusters find their places late: 33 rows
-  // of 4096 x 4096 12.6 us with the launch, 9.3 here, of K 16384, N 2048 11.0 and 20.
+  // of 4096 x 4096 (K 1024, N 1024) 7.3 us (4.7) there and 6.3 (3.4) here, 32 rows 6.0 (4.1), 16 rows 5.2 (3.7), 64 rows of K
+  // 16384, N 2048 8.1 and 13.6, 128 rows of it 15.7 and 16.8.  Behind a quantizing launch its clusters find their places
+  // late: 33 rows of 4096 x 4096 12.6 us with the launch, 9.0 here, of K 16384, N 2048 11.0 and 19.
   const int64_t k_blocks = (K + 255) / 256;
-  if ((M <= 16 && !quantized) || (M <= 64 && k_blocks >= 8 && !quantized) || (M <= kFewRows && k_blocks >= 32))
+  if ((M <= 16 && !quantized) || (M <= 32 && k_blocks >= 16 && !quantized) || (M <= kFewRows && k_blocks >= 32))
     return run_fp4_few_rows(fc_params(out, bias, M, K, N, flags, status), out_type, a, sa, -1, 0, b, sb, K, s);
   const FcParams p = fc_params(out, bias, M, K, N, flags, status);
   return with_float_type(out_type, [&](auto *t) {

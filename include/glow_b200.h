@@ -670,8 +670,8 @@ int glowb200_microscaled_fp4_dequantize(const uint8_t *data, const uint8_t *scal
 
 /* Fully connected layer over microscaled operands: out[i,j] = sum_k in[i,k] * weights[j,k] + bias[j], fp32 sums, rounded
  * to out_type once.  in [M,K] and weights [N,K] in the format above; bias fp32 [N] or NULL; out [M,N] dense.
- * flags: GLOWB200_FC_FUSE_RELU (NaN stays NaN).  The bytes behind column K are read: they are zeros, as the quantizer
- * leaves them. */
+ * flags: GLOWB200_FC_FUSE_RELU (NaN stays NaN).  Data and scale bytes behind column K are read: they are zeros, as the
+ * quantizer leaves them. */
 int glowb200_microscaled_fp4_fc(void *out, int out_type, const uint8_t *in, const uint8_t *in_scales, const uint8_t *weights,
                                 const uint8_t *weights_scales, const float *bias, int64_t M, int64_t K, int64_t N, int flags,
                                 int32_t *status, glowb200_stream_t stream);

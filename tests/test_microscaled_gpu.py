@@ -194,6 +194,23 @@ def test_dynamic_fc_is_quantize_and_fc(M, K, N, dtype):
     assert int(st.item()) == 0
 
 
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("M,K,N", [(1, 4096, 16500), (1, 9000, 2500), (1, 20000, 300), (2, 9000, 2500), (3, 8200, 9600), (5, 6000, 9600), (7, 9000, 2500),
+                                   (16, 12000, 700), (20, 5000, 5000), (32, 20000, 300)])
+def test_dynamic_fc_of_long_rows(M, K, N, dtype):
+    """More k-blocks to a block than its ring holds, twice over and more, for every way of dealing rows to warps."""
+    g = torch.Generator(device=DEV).manual_seed(M + K)
+    x = torch.randn(M, K, device=DEV, generator=g).to(TYPES[dtype])
+    w, ws = ops.microscaled_fp4_quantize(torch.randn(N, K, device=DEV, generator=g))
+    st = ops.new_status(DEV)
+    got = ops.dynamic_microscaled_fp4_fc(x, w, ws, out_dtype=torch.float32, status=st)
+    va, vb = (ops.microscaled_fp4_dequantize(d, s, K).double() for d, s in (ops.microscaled_fp4_quantize(x), (w, ws)))
+    assert ((got.double() - va @ vb.T).abs() <= (K + 1) * 2.0 ** -23 * (va.abs() @ vb.abs().T)).all()
+    # rows of ones: sums of the weights, multiples of 2^-8 below 2^16 here, exact in fp32 whatever their order
+    assert torch.equal(ops.dynamic_microscaled_fp4_fc(torch.ones_like(x), w, ws, out_dtype=torch.float32).double()[-1], vb.sum(1))
+    assert int(st.item()) == 0
+
+
 def test_dynamic_fc_with_rows_apart_and_a_given_workspace():
     whole = rows_of(3, 20, 300, "fp16").to(DEV)
     x = whole[:, 10:266]
