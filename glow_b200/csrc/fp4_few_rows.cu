@@ -4,7 +4,11 @@
 // are computed for a token.  What bounds such a product is the weights' bytes and, at these sizes, latency: the depth is
 // split over the blocks of a cluster, each of which has its k-blocks on their way at once, and their sums meet in shared
 // memory, added in the blocks' order.  A float input is quantized by the block's own warps on its way to shared memory
-// (4 warps, 256 columns of a row to a warp at a time): a launch of its own would cost more than the work does.
+// (eight warps, 256 columns of a row to a warp at a time): a launch of its own would cost more than the work does.
+//
+// One row of 4096 x 4096 takes 4.5 us, 8 float rows 5.3: 2.7 us are a launch's chain of map, load, scales, MMA and drain with
+// one k-block, 0.9 a cluster's two barriers, the rest k-blocks, whose instructions take 0.2 us to issue.  The weights' bytes
+// would take 1.4.  One row of K 4096, N 16384 moves 36 MB in 6.2 us, 5.8 TB/s.
 #include "fp4_mma.cuh"
 
 namespace glowb200 {

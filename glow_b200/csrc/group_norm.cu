@@ -8,10 +8,17 @@
 //   M2 = M2a + M2b + (mean_b - mean_a)^2 na nb / (na + nb),
 // in an order that depends on the sizes alone.
 //
-// Bound by bytes, or by launches.  Small inputs take one launch: a block has some groups of one image and reads their
-// pixels twice, the second time from cache.  Others take two: statistics of chunks of pixels, all channels to a block, then
-// a pass that joins them and normalises, from the last chunk to the first: what the first pass read last is still in L2
-// (126 MB).
+// Three ways, by size:
+//   - one launch (norm_single_kernel) where a slice of 64 bytes of every pixel, whole groups, of one image lies in the shared
+//     memory of one to eight blocks: they form a cluster, tell one another what they know of the groups, and read their
+//     pixels once.  Bound by latency (one image of 14 x 14 x 1024 fp16: 4.0 us) or by issue slots: some 70 instructions to
+//     16 bytes and 590 to a warp beside them (64 x 56 x 56 x 256 fp16 48 us, 4.3 TB/s of 205 MB that have to move; its two
+//     launches 60).  128 bytes of a pixel take 52 there, 32 bytes 56, twice the blocks 57.
+//   - two launches (norm_stats_kernel, norm_chunks_kernel) for larger images: statistics of chunks of whole pixels, then a
+//     pass that joins them and normalises, from the last chunk and the last pixels to the first: what the first pass read
+//     last is still in L2 (126 MB).  Bound by bytes: 8 x 256 x 256 x 128 fp16 70 us, of which the statistics take 24 (134 MB at
+//     5.6 TB/s) and the rest moves 268 MB through L2 at the rate of a copy; Swish adds 5.
+//   - any number of channels a pixel (norm_any_*): three plain launches.
 #include "microscaled.cuh"
 #include "tcgen05.cuh"
 
