@@ -750,8 +750,8 @@ int side_by_side(const void *in, const void *out, int in_bytes, int out_bytes, i
 // Channels of a slice of the single launch: the fewest whole groups of 64 bytes or more a pixel.  0: none suits.
 int64_t pick_slice(int64_t channels, int64_t groups, int vec, int in_bytes) {
   const int64_t width = channels / groups;
-  for (int64_t k = 1; k <= groups; k++)
-    if (groups % k == 0 && width * k % vec == 0 && (width * k * in_bytes >= 64 || k == groups)) return width * k / vec <= kNormThreads ? width * k : 0;
+  for (int64_t k = 1; k <= groups && width * k / vec <= kNormThreads; k++)
+    if (groups % k == 0 && width * k % vec == 0 && (width * k * in_bytes >= 64 || k == groups)) return width * k;
   return 0;
 }
 

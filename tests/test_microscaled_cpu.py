@@ -1,5 +1,6 @@
 """The microscaled 4-bit entry points and group norm turn down on the host what they cannot take; no GPU is needed."""
 import ctypes as C
+import time
 
 import numpy as np
 import pytest
@@ -71,6 +72,14 @@ def test_group_norm_refuses(l, change, code):
     v.update(change)
     assert l.glowb200_group_norm(*v.values(), None, None) == code
     assert l.glowb200_last_error()
+
+
+def test_group_norm_plans_any_number_of_groups_at_once(l):
+    """A prime number of groups has no whole number of groups in a slice: the search for one ends early (2^31 steps take seconds)."""
+    prime = 2**31 - 1
+    start = time.perf_counter()
+    assert l.glowb200_group_norm_workspace_bytes(1, 1, prime, prime) > 8 * prime
+    assert time.perf_counter() - start < 1
 
 
 def test_the_reference_itself():
