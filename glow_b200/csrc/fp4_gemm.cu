@@ -416,6 +416,15 @@ int check_fc(const void *out, int out_type, const void *in, const void *weights,
   return GLOWB200_OK;
 }
 
+// The result beside weights and bias.
+int check_beside(const void *out, int out_type, const void *weights, const void *weights_scales, const float *bias, int64_t M, int64_t K, int64_t N) {
+  const size_t bytes = (size_t)(M * N) * float_type_bytes(out_type);
+  GLOWB200_REQUIRE(apart(out, bytes, weights, (size_t)(N * mx_pitch(K))) && apart(out, bytes, weights_scales, glowb200_microscaled_fp4_scales_bytes(N, K)) &&
+                       (bias == nullptr || apart(out, bytes, bias, (size_t)N * 4)),
+                   "the result lies over the weights or the bias");
+  return GLOWB200_OK;
+}
+
 FcParams fc_params(void *out, const float *bias, int64_t M, int64_t K, int64_t N, int flags, int32_t *status) {
   return {out, bias, status, (int)M, (int)N, (int)((K + 63) / 64), (flags & GLOWB200_FC_FUSE_RELU) != 0, 0};
 }
@@ -447,6 +456,10 @@ extern "C" int glowb200_microscaled_fp4_fc(void *out, int out_type, const uint8_
   if (M == 0 || N == 0) return GLOWB200_OK;
   GLOWB200_REQUIRE(in_scales, "NULL tensor pointer");
   GLOWB200_REQUIRE(aligned(in, 16) && aligned(in_scales, 16), "data and scales must start on 16-byte boundaries");
+  const size_t out_bytes = (size_t)(M * N) * float_type_bytes(out_type);
+  GLOWB200_REQUIRE(apart(out, out_bytes, in, (size_t)(M * mx_pitch(K))) && apart(out, out_bytes, in_scales, glowb200_microscaled_fp4_scales_bytes(M, K)),
+                   "the result lies over the input");
+  if (int rc = check_beside(out, out_type, weights, weights_scales, bias, M, K, N)) return rc;
   return run_fc(out, out_type, in, in_scales, weights, weights_scales, bias, M, K, N, flags, status, false,
                 reinterpret_cast<cudaStream_t>(stream));
 }
@@ -469,6 +482,12 @@ extern "C" int glowb200_dynamic_microscaled_fp4_fc(void *out, int out_type, cons
   if (workspace == nullptr || workspace_bytes < need)
     return set_error(GLOWB200_ERR_WORKSPACE_TOO_SMALL, "workspace of %zu bytes given, %zu needed", workspace_bytes, need);
   GLOWB200_REQUIRE(aligned(workspace, 256), "workspace must be 256-byte aligned");
+  const size_t out_bytes = (size_t)(M * N) * float_type_bytes(out_type), row_bytes = (size_t)K * float_type_bytes(in_type),
+               stride_bytes = (size_t)row_stride * float_type_bytes(in_type);
+  GLOWB200_REQUIRE(apart(out, out_bytes, in, row_bytes, M, stride_bytes) && apart(out, out_bytes, workspace, need) &&
+                       apart(workspace, need, in, row_bytes, M, stride_bytes),
+                   "result, input and workspace lie over one another");
+  if (int rc = check_beside(out, out_type, weights, weights_scales, bias, M, K, N)) return rc;
   // Every tile of 128 columns quantizes all rows for itself: 8 rows of N 16384 8.6 us, in two launches 10; 16 rows 12.5 and
   // 10.4; 32 rows of N 4096 9.2 and 9.2.
   if (M <= kFewQuantizedRows && M * ((N + 127) / 128) <= 1024)

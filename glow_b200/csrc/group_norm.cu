@@ -895,6 +895,14 @@ extern "C" int glowb200_group_norm(void *out, int out_type, int8_t *out_i8, floa
   if (need > 0 && (workspace == nullptr || workspace_bytes < need))
     return set_error(GLOWB200_ERR_WORKSPACE_TOO_SMALL, "workspace of %zu bytes given, %zu needed", workspace_bytes, need);
   GLOWB200_REQUIRE(aligned(workspace, 256), "workspace must be 256-byte aligned");
+  const void *result = out_i8 != nullptr ? out_i8 : out;
+  const int in_bytes = float_type_bytes(in_type), out_bytes = out_i8 != nullptr ? 1 : float_type_bytes(out_type);
+  const size_t count = (size_t)(images * pixels * channels);
+  GLOWB200_REQUIRE((result == in && in_bytes == out_bytes) || apart(result, count * out_bytes, in, count * in_bytes), "the result lies over a part of the input");
+  GLOWB200_REQUIRE((gamma == nullptr || apart(result, count * out_bytes, gamma, (size_t)channels * 4)) &&
+                       (beta == nullptr || apart(result, count * out_bytes, beta, (size_t)channels * 4)) &&
+                       (need == 0 || (apart(workspace, need, in, count * in_bytes) && apart(workspace, need, result, count * out_bytes))),
+                   "the result or the workspace lies over another tensor");
   NormParams p{};
   p.in = in, p.out = out, p.out_i8 = out_i8, p.gamma = gamma, p.beta = beta;
   p.stats = reinterpret_cast<float2 *>(workspace);

@@ -252,6 +252,10 @@ extern "C" int glowb200_microscaled_fp4_quantize(const void *in, int in_type, in
   GLOWB200_REQUIRE(in && data && scales, "NULL tensor pointer");
   GLOWB200_REQUIRE(aligned(in, float_type_bytes(in_type)), "the input is not aligned to its elements");
   GLOWB200_REQUIRE(aligned(data, 16) && aligned(scales, 16), "data and scales must start on 16-byte boundaries");
+  const size_t bytes = (size_t)float_type_bytes(in_type), data_bytes = (size_t)(rows * mx_pitch(cols)), scale_bytes = glowb200_microscaled_fp4_scales_bytes(rows, cols);
+  GLOWB200_REQUIRE(apart(data, data_bytes, in, cols * bytes, rows, row_stride * bytes) && apart(scales, scale_bytes, in, cols * bytes, rows, row_stride * bytes) &&
+                       apart(data, data_bytes, scales, scale_bytes),
+                   "a result lies over the input or the other result");
   return run_mx_quantize(in, in_type, rows, cols, row_stride, data, scales, reinterpret_cast<cudaStream_t>(stream));
 }
 
@@ -263,6 +267,9 @@ extern "C" int glowb200_microscaled_fp4_dequantize(const uint8_t *data, const ui
   GLOWB200_REQUIRE(data && scales && out, "NULL tensor pointer");
   GLOWB200_REQUIRE(aligned(data, 16) && aligned(scales, 16), "data and scales must start on 16-byte boundaries");
   GLOWB200_REQUIRE(aligned(out, float_type_bytes(out_type)), "the result is not aligned to its elements");
+  const size_t out_bytes = (size_t)(rows * cols) * float_type_bytes(out_type);
+  GLOWB200_REQUIRE(apart(out, out_bytes, data, (size_t)(rows * mx_pitch(cols))) && apart(out, out_bytes, scales, glowb200_microscaled_fp4_scales_bytes(rows, cols)),
+                   "the result lies over the input");
   const int64_t tiles = mx_tiles(cols), blocks = mx_row_tiles(rows) * tiles;
   GLOWB200_REQUIRE(blocks < (1ll << 31), "the matrix has more than 2^31 tiles of 128 x 128");
   return with_float_type(out_type, [&](auto *t) {

@@ -15,6 +15,13 @@ inline int64_t mx_tiles(int64_t cols) { return (mx_blocks(cols) + 3) / 4; }    /
 inline int64_t mx_row_tiles(int64_t rows) { return (rows + 127) / 128; }
 
 inline bool aligned(const void *p, size_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
+// Whether `n` bytes at p lie beside all of `rows` rows of `m` bytes, `stride` bytes apart, from q on.
+inline bool apart(const void *p, size_t n, const void *q, size_t m, size_t rows = 1, size_t stride = 0) {
+  const uintptr_t a = reinterpret_cast<uintptr_t>(p), b = reinterpret_cast<uintptr_t>(q);
+  if (a < b) return n <= b - a;
+  const size_t row = rows > 1 ? (a - b) / stride : 0, at = a - b - row * stride;  // in front of the first byte
+  return row >= rows || (at >= m && (row + 1 >= rows || n <= stride - at));
+}
 inline int float_type_bytes(int type) { return type == GLOWB200_FLOAT32 ? 4 : 2; }
 // Calls f with a null pointer of the element type behind GLOWB200_FLOAT32 / FLOAT16 / BFLOAT16.
 template <typename F>

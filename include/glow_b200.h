@@ -658,7 +658,9 @@ int glowb200_quantize_transpose_i8(int8_t *dest, const float *src, const int64_t
  *           blocks, 512 bytes each: row r, block b is byte (r % 32) * 16 + (r / 32 % 4) * 4 + b % 4 of tile
  *           (r / 128) * ceil(blocks / 4) + b / 4.  Bytes of rows and blocks that are not there are 0.
  * Both start on 16-byte boundaries.  A block that holds a NaN or an infinity has the scale byte 255 and stands for 32
- * NaNs.  This tile order is the one in which the tensor cores take the scales. */
+ * NaNs.  This tile order is the one in which the tensor cores take the scales.
+ * In this section a result or a workspace that lies over an operand, or one over the other, is an invalid argument (but
+ * group norm's result may be its input). */
 size_t glowb200_microscaled_fp4_scales_bytes(int64_t rows, int64_t cols);
 /* in [rows, cols] of in_type, rows `row_stride` elements apart (at least cols). */
 int glowb200_microscaled_fp4_quantize(const void *in, int in_type, int64_t rows, int64_t cols, int64_t row_stride,
@@ -690,7 +692,7 @@ int glowb200_dynamic_microscaled_fp4_fc(void *out, int out_type, const void *in,
  *   y = act((x - mean) / sqrt(variance + eps) * gamma[c] + beta[c])
  * gamma, beta: fp32 [channels] or NULL (1 and 0).  The result, dense like `in`, is rounded once to out_type, or to int8
  * as glowb200_element_quantize_i8 does it with quant_scale / quant_offset: exactly one of out and out_i8 is given.
- * act: GLOWB200_NORM_ACT_*.  `out` may be `in`.  The workspace (256-byte aligned) must hold
+ * act: GLOWB200_NORM_ACT_*.  `out` may be `in` where their types have one size.  The workspace (256-byte aligned) must hold
  * glowb200_group_norm_workspace_bytes(...) bytes; small images need none. */
 #define GLOWB200_NORM_ACT_NONE 0
 #define GLOWB200_NORM_ACT_RELU 1

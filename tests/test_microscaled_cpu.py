@@ -74,6 +74,42 @@ def test_group_norm_refuses(l, change, code):
     assert l.glowb200_last_error()
 
 
+def at(n):
+    return C.c_void_p(1 << 20 | n)
+
+
+def over(l, code):
+    return code == 1 and b" over " in l.glowb200_last_error()
+
+
+def test_results_over_operands_are_refused(l):
+    """Addresses are never read: these calls end on the host."""
+    far, q = C.c_void_p(1 << 24), l.glowb200_microscaled_fp4_quantize
+    # 4 rows of 64 floats (256 bytes), 512 bytes apart: bytes 0-255, 512-767, ...; data 128 bytes, scales 512
+    for data in (0, 255 // 16 * 16, 512, 1536, 464, 1776):  # (464: its last bytes reach row 1; 1776: the last row's last ones)
+        assert over(l, q(at(0), 0, 4, 64, 128, at(data), far, None)), data
+    assert over(l, q(at(4096), 0, 4, 64, 64, at(4096 - 112), far, None)) and over(l, q(at(0), 0, 4, 64, 128, far, at(256), None))
+    assert over(l, q(at(0), 0, 4, 64, 64, far, C.c_void_p((1 << 24) + 112), None))
+    assert over(l, l.glowb200_microscaled_fp4_dequantize(at(0), far, 4, 64, at(64), 0, None))
+    assert over(l, l.glowb200_microscaled_fp4_dequantize(far, at(0), 4, 64, at(508), 0, None))
+    for k in range(2, 7):  # the result (128 bytes) at each operand's last bytes in turn
+        args = [at(0), 0] + [C.c_void_p((1 << 24) + 4096 * i) for i in range(5)] + [4, 64, 8, 0, None, None]
+        args[0] = C.c_void_p(args[k].value + 28)
+        assert over(l, l.glowb200_microscaled_fp4_fc(*args)), k
+    d = l.glowb200_dynamic_microscaled_fp4_fc
+    far2, far3 = C.c_void_p(1 << 25), C.c_void_p(1 << 26)
+    assert over(l, d(at(0), 0, at(0), 0, 64, far, far2, None, 4, 64, 64, 0, far3, 1 << 20, None, None))
+    assert over(l, d(at(0), 0, far3, 0, 64, far, far2, None, 4, 64, 64, 0, at(512), 1 << 20, None, None))
+    assert over(l, d(at(0), 0, far3, 0, 64, far, far2, None, 4, 64, 64, 0, far3, 1 << 20, None, None))
+    assert over(l, d(far2, 0, far3, 0, 64, far, far2, None, 4, 64, 64, 0, at(0), 1 << 20, None, None))
+
+    def norm(out, inp, out_type=1, out_i8=None, gamma=None, ws=None, pixels=9):
+        return l.glowb200_group_norm(out, out_type, out_i8, 1.0, 0, inp, 1, gamma, None, 2, pixels, 8, 2, 1e-5, 0, ws, 1 << 20, None, None)
+    assert over(l, norm(at(2), at(0))) and over(l, norm(at(0), at(2))) and over(l, norm(at(0), at(0), out_type=0))
+    assert over(l, norm(None, at(0), out_i8=at(0))) and over(l, norm(at(0), at(0), gamma=at(4)))
+    assert over(l, norm(far, at(0), ws=at(0), pixels=1 << 20)) and over(l, norm(far, far2, ws=far, pixels=1 << 16))
+
+
 def test_group_norm_plans_any_number_of_groups_at_once(l):
     """A prime number of groups has no whole number of groups in a slice: the search for one ends early (2^31 steps take seconds)."""
     prime = 2**31 - 1

@@ -82,6 +82,15 @@ def test_quantize_rows_that_are_apart(cols, start, stride, dtype):
     check_format(x, data, scales)
 
 
+def test_results_between_rows_that_are_apart():
+    """A result may lie where the input's rows leave room."""
+    buf = torch.randn(3, 4096, device=DEV)
+    x, want = buf[:, :64], ops.microscaled_fp4_quantize(buf[:, :64].contiguous())
+    data, scales = buf[0, 64:].view(torch.uint8)[:96].view(3, 32), buf[1, 64:].view(torch.uint8)[:512].view(1, 1, 512)
+    ops.microscaled_fp4_quantize(x, out=data, scales=scales)
+    assert torch.equal(data, want[0]) and torch.equal(scales, want[1])
+
+
 @pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
 def test_extreme_numbers(dtype):
     fi = torch.finfo(TYPES[dtype])
