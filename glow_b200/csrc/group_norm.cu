@@ -19,13 +19,13 @@
 //     last is still in L2 (126 MB).  Bound by bytes: 8 x 256 x 256 x 128 fp16 70 us, of which the statistics take 24 (134 MB at
 //     5.6 TB/s) and the rest moves 268 MB through L2 at the rate of a copy; Swish adds 5.
 //   - any number of channels a pixel (norm_any_*): three plain launches.
+#include "group_norm_plan.h"
 #include "microscaled.cuh"
 #include "tcgen05.cuh"
 
 namespace glowb200 {
 namespace {
 
-constexpr int kNormThreads = 512;
 constexpr int kMostShared = 232448;  // bytes that a block can have: what kernels are allowed, whatever a launch takes (calls may overlap)
 
 struct NormParams {
@@ -260,9 +260,8 @@ struct Loads {
   }
 };
 
-// The same for at most kHeld pixels of a thread that stay in shared memory, so that they come from memory once: asynchronous
+// The same for at most kNormHeld pixels of a thread that stay in shared memory, so that they come from memory once: asynchronous
 // copies of 16 bytes, four commit groups of four (each thread reads what it copied itself).
-constexpr int kHeld = 16;
 template <typename T, int VEC>
 struct Held {
   static constexpr bool kCan = VEC * sizeof(T) == 16;
@@ -275,7 +274,7 @@ struct Held {
       : place((uint32_t)__cvta_generic_to_shared(shared) + 16 * threadIdx.x), left(from.left), first(true) {
     const T *at = from.at;
 #pragma unroll
-    for (int g = 0; g < kHeld / kBatch; g++) {
+    for (int g = 0; g < kNormHeld / kBatch; g++) {
 #pragma unroll
       for (int i = 0; i < kBatch; i++)
         if (g * kBatch + i < left) {
@@ -747,26 +746,12 @@ int side_by_side(const void *in, const void *out, int in_bytes, int out_bytes, i
     if (vec > 1 && channels % vec == 0 && aligned(in, vec * in_bytes) && aligned(out, vec * out_bytes > 16 ? 16 : vec * out_bytes)) return vec;
   return 1;
 }
-// Channels of a slice of the single launch: the fewest whole groups of 64 bytes or more a pixel.  0: none suits.
-int64_t pick_slice(int64_t channels, int64_t groups, int vec, int in_bytes) {
-  const int64_t width = channels / groups;
-  for (int64_t k = 1; k <= groups && width * k / vec <= kNormThreads; k++)
-    if (groups % k == 0 && width * k % vec == 0 && (width * k * in_bytes >= 64 || k == groups)) return width * k;
-  return 0;
-}
-
-// Pixels that a block takes side by side: of 256 threads' pieces; 512 where a pixel has more, 128 where those hold a whole slice
-// (64 x 7 x 7 x 2048 17.6 -> 10.2 us, one image of 14 x 14 x 1024 4.2 -> 4.0; in clusters 8 x 28 x 28 x 512 6.0 -> 6.4).
-int rows_for(int64_t columns, int64_t pixels) {
-  const int64_t rows = (columns <= 64 && columns * pixels <= 128 * (kHeld - 1) ? 128 : columns <= 256 ? 256 : kNormThreads) / columns;
-  return (int)(rows < pixels ? rows : pixels);
-}
 
 template <typename T, int VEC, int UNIT, typename Out>
 int launch_unit(NormParams p, int64_t slice, cudaStream_t s) {
   const int width = p.channels / p.groups;
   const int64_t columns = (slice > 0 ? slice : p.channels) / VEC;
-  p.rows = rows_for(columns, p.chunk_pixels);
+  if (slice == 0) p.rows = norm_rows(columns, p.chunk_pixels);
   auto reciprocal = [](int64_t d) { return 0xffffffffu / (uint32_t)d; };
   p.width = width, p.columns = (int)columns, p.of_group = width / UNIT;
   p.by_width = reciprocal(width), p.by_columns = reciprocal(columns), p.by_rows = reciprocal(p.rows), p.by_group = reciprocal(p.of_group);
@@ -778,6 +763,7 @@ int launch_unit(NormParams p, int64_t slice, cudaStream_t s) {
     const size_t own = parts + 2 * (size_t)(slice / width) * sizeof(float2);
     p.held_at = (int)align_up(own, 16);
     const int64_t each = (p.chunk_pixels + p.rows - 1) / p.rows;
+    GLOWB200_REQUIRE(each <= kNormHeld, "more pixels to a thread than stay in shared memory");
     const size_t shared = Held<T, VEC>::kCan ? p.held_at + Held<T, VEC>::bytes((int)threads, (int)align_up((size_t)each, 4)) : own;
     auto kernel = norm_single_kernel<T, VEC, UNIT, Out>;
     GLOWB200_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostShared));
@@ -822,30 +808,14 @@ int launch_width(const NormParams &p, int vec, int64_t slice, cudaStream_t s) {
   else return vec == 8 ? launch_vec<T, 8, Out>(p, slice, s) : launch_vec<T, 2, Out>(p, slice, s);
 }
 
-// Blocks of the one launch's clusters: as few as hold a slice's pixels, eight at most; 0: they do not.
-int64_t single_blocks(int64_t slice, int vec, int64_t pixels) {
-  if (slice <= 0) return 0;
-  const int64_t most = (int64_t)rows_for(slice / vec, pixels) * (kHeld - 1);
-  for (int64_t blocks = 1; blocks <= 8; blocks *= 2)
-    if (blocks * most >= pixels) return blocks;
-  return 0;
-}
-// Whether every type and alignment of such an input takes the one launch, which needs no workspace.
-bool always_single(int64_t pixels, int64_t channels, int64_t groups) {
-  for (int bytes : {2, 4})
-    for (int vec : {16 / bytes, 4 / bytes, 1})
-      if (channels % vec == 0 && single_blocks(pick_slice(channels, groups, vec, bytes), vec, pixels) == 0) return false;
-  return true;
-}
-
 template <typename T, typename Out>
 int launch(NormParams p, cudaStream_t s) {
   const void *out = sizeof(Out) == 1 ? static_cast<const void *>(p.out_i8) : p.out;
   const int vec = side_by_side(p.in, out, sizeof(T), sizeof(Out), p.channels);
-  const int64_t slice = pick_slice(p.channels, p.groups, vec, sizeof(T)), blocks_of_slice = single_blocks(slice, vec, p.pixels);
-  if (blocks_of_slice > 0) {
-    p.chunks = (int)blocks_of_slice;
-    p.chunk_pixels = (p.pixels + blocks_of_slice - 1) / blocks_of_slice;
+  const int64_t slice = norm_slice(p.channels, p.groups, vec, sizeof(T));
+  const NormSingle single = norm_single(slice, vec, p.pixels);
+  if (single.blocks > 0) {
+    p.chunks = single.blocks, p.rows = single.rows, p.chunk_pixels = single.chunk_pixels;
     return launch_width<T, Out>(p, vec, slice, s);
   }
   if (p.channels / vec <= kNormThreads) {
@@ -871,7 +841,7 @@ using namespace glowb200;
 
 extern "C" size_t glowb200_group_norm_workspace_bytes(int64_t images, int64_t pixels, int64_t channels, int64_t groups) {
   if (images <= 0 || pixels <= 0 || channels <= 0 || groups <= 0) return 0;
-  if (channels % groups != 0 || always_single(pixels, channels, groups)) return 0;
+  if (channels % groups != 0 || norm_always_single(pixels, channels, groups)) return 0;
   const int64_t a = any_chunks(images, pixels, channels, groups), b = image_chunks(images, pixels, channels);
   return align_up((size_t)(images * groups) * 8, 256) + (size_t)(images * groups * (a > b ? a : b)) * 8;
 }

@@ -207,3 +207,17 @@ def test_a_block_of_layers(oracle):
     y, size = va @ vb.T + bias.double(), va.abs() @ vb.abs().T + bias.abs().double()
     off = (got.view(-1, OC).double() - y.clamp(min=0)).abs()
     assert (off <= (C + 2) * 2.0 ** -23 * size * (1 + 2.0 ** -11) + 2.0 ** -11 * y.abs() + 2.0 ** -24).all()
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "fp16", "bf16"])
+@pytest.mark.parametrize("shape,G", [((1, 14, 14, 608), 32), ((2, 17, 17, 104), 8), ((1, 17, 17, 416), 32), ((3, 14, 14, 152), 1), ((1, 12, 12, 208), 1),
+                                     ((2, 8, 10, 384), 1), ((2, 8, 10, 192), 1), ((1, 13, 12, 1536), 4), ((1, 34, 34, 104), 8), ((1, 24, 24, 52), 4)])
+def test_slices_whose_pieces_do_not_divide_a_block(shape, G, dtype):
+    """Slices of 13, 19, 26, 48 and more pieces of 16 bytes over clusters, in shared memory that another norm has filled with
+    large numbers: a pixel that is not copied there would count with one of those."""
+    ops.group_norm(torch.full((64, 56, 56, 256), 6e4, dtype=torch.float16, device=DEV), 32)
+    x, gamma, beta = case(shape[-1] + 2 * G, shape, dtype)
+    got = ops.group_norm(x, G, gamma, beta)
+    y, off = wanted(x, G, gamma, beta, 1e-5, "none", torch.finfo(x.dtype).eps / 2)
+    tiny = torch.finfo(x.dtype).smallest_normal * torch.finfo(x.dtype).eps
+    assert ((got.double() - y).abs() <= off + tiny).all()
