@@ -416,12 +416,11 @@ int check_fc(const void *out, int out_type, const void *in, const void *weights,
   return GLOWB200_OK;
 }
 
-// The result beside weights and bias.
-int check_beside(const void *out, int out_type, const void *weights, const void *weights_scales, const float *bias, int64_t M, int64_t K, int64_t N) {
-  const size_t bytes = (size_t)(M * N) * float_type_bytes(out_type);
-  GLOWB200_REQUIRE(apart(out, bytes, weights, (size_t)(N * mx_pitch(K))) && apart(out, bytes, weights_scales, glowb200_microscaled_fp4_scales_bytes(N, K)) &&
-                       (bias == nullptr || apart(out, bytes, bias, (size_t)N * 4)),
-                   "the result lies over the weights or the bias");
+// What is written (`name`: n bytes at p) beside weights and bias.
+int check_beside(const char *name, const void *p, size_t n, const void *weights, const void *weights_scales, const float *bias, int64_t K, int64_t N) {
+  GLOWB200_REQUIRE(apart(p, n, weights, (size_t)(N * mx_pitch(K))) && apart(p, n, weights_scales, glowb200_microscaled_fp4_scales_bytes(N, K)) &&
+                       (bias == nullptr || apart(p, n, bias, (size_t)N * 4)),
+                   "the %s lies over the weights or the bias", name);
   return GLOWB200_OK;
 }
 
@@ -459,7 +458,7 @@ extern "C" int glowb200_microscaled_fp4_fc(void *out, int out_type, const uint8_
   const size_t out_bytes = (size_t)(M * N) * float_type_bytes(out_type);
   GLOWB200_REQUIRE(apart(out, out_bytes, in, (size_t)(M * mx_pitch(K))) && apart(out, out_bytes, in_scales, glowb200_microscaled_fp4_scales_bytes(M, K)),
                    "the result lies over the input");
-  if (int rc = check_beside(out, out_type, weights, weights_scales, bias, M, K, N)) return rc;
+  if (int rc = check_beside("result", out, out_bytes, weights, weights_scales, bias, K, N)) return rc;
   return run_fc(out, out_type, in, in_scales, weights, weights_scales, bias, M, K, N, flags, status, false,
                 reinterpret_cast<cudaStream_t>(stream));
 }
@@ -487,7 +486,8 @@ extern "C" int glowb200_dynamic_microscaled_fp4_fc(void *out, int out_type, cons
   GLOWB200_REQUIRE(apart(out, out_bytes, in, row_bytes, M, stride_bytes) && apart(out, out_bytes, workspace, need) &&
                        apart(workspace, need, in, row_bytes, M, stride_bytes),
                    "result, input and workspace lie over one another");
-  if (int rc = check_beside(out, out_type, weights, weights_scales, bias, M, K, N)) return rc;
+  if (int rc = check_beside("result", out, out_bytes, weights, weights_scales, bias, K, N)) return rc;
+  if (int rc = check_beside("workspace", workspace, need, weights, weights_scales, bias, K, N)) return rc;
   // Every tile of 128 columns quantizes all rows for itself: 8 rows of N 16384 8.6 us, in two launches 10; 16 rows 12.5 and
   // 10.4; 32 rows of N 4096 9.2 and 9.2.
   if (M <= kFewQuantizedRows && M * ((N + 127) / 128) <= 1024)

@@ -127,3 +127,19 @@ def test_the_reference_itself():
     assert list(ref.values(codes, sc)[0, :10]) == [6, 4, 2, -4, 0, 1, 0, 1, 2, 6]
     assert list(ref.values(codes, sc)[0, 32:34]) == [8, -3] and list(sc[0]) == [127, 128]
     assert codes[0, 6] == 8  # -0.2 becomes -0
+
+
+@pytest.mark.parametrize("rows", [4, 40, 200])
+def test_a_workspace_over_weights_or_bias_is_refused(l, rows):
+    """The quantized input goes through the workspace: over the weights it would be multiplied with itself, and they would be gone."""
+    names, size = ("out", "inp", "weights", "weights_scales", "bias", "ws"), 1 << 22
+    need = l.glowb200_dynamic_microscaled_fp4_fc_workspace_bytes(rows, 64, 512)
+    for name, last in (("weights", 512 * 32), ("weights_scales", 4 * 512), ("bias", 2048)):
+        # on the operand, on its last bytes, and with its own last bytes on the operand's first
+        for move in (0, last - 256, -((need - 1) // 256 * 256)):
+            v = {n: size * (i + 1) for i, n in enumerate(names)}
+            v["ws"] = v[name] + move
+            a = {n: C.c_void_p(p) for n, p in v.items()}
+            rc = l.glowb200_dynamic_microscaled_fp4_fc(a["out"], 0, a["inp"], 0, 64, a["weights"], a["weights_scales"], a["bias"], rows, 64, 512, 0,
+                                                       a["ws"], 1 << 20, None, None)
+            assert over(l, rc), (name, move)
