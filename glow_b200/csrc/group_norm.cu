@@ -871,7 +871,9 @@ extern "C" int glowb200_group_norm(void *out, int out_type, int8_t *out_i8, floa
   GLOWB200_REQUIRE((result == in && in_bytes == out_bytes) || apart(result, count * out_bytes, in, count * in_bytes), "the result lies over a part of the input");
   GLOWB200_REQUIRE((gamma == nullptr || apart(result, count * out_bytes, gamma, (size_t)channels * 4)) &&
                        (beta == nullptr || apart(result, count * out_bytes, beta, (size_t)channels * 4)) &&
-                       (need == 0 || (apart(workspace, need, in, count * in_bytes) && apart(workspace, need, result, count * out_bytes))),
+                       (need == 0 || (apart(workspace, need, in, count * in_bytes) && apart(workspace, need, result, count * out_bytes) &&
+                                      (gamma == nullptr || apart(workspace, need, gamma, (size_t)channels * 4)) &&
+                                      (beta == nullptr || apart(workspace, need, beta, (size_t)channels * 4)))),
                    "the result or the workspace lies over another tensor");
   NormParams p{};
   p.in = in, p.out = out, p.out_i8 = out_i8, p.gamma = gamma, p.beta = beta;

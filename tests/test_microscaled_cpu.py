@@ -143,3 +143,13 @@ def test_a_workspace_over_weights_or_bias_is_refused(l, rows):
             rc = l.glowb200_dynamic_microscaled_fp4_fc(a["out"], 0, a["inp"], 0, 64, a["weights"], a["weights_scales"], a["bias"], rows, 64, 512, 0,
                                                        a["ws"], 1 << 20, None, None)
             assert over(l, rc), (name, move)
+
+
+def test_a_workspace_over_gamma_or_beta_is_refused(l):
+    pixels, far, far2 = 1 << 20, C.c_void_p(1 << 30), C.c_void_p(1 << 40)
+    need = l.glowb200_group_norm_workspace_bytes(2, pixels, 64, 8)
+    for gamma, beta in ((1 << 20, None), (None, 1 << 20), (1 << 28, 1 << 20)):
+        g, b = (None if v is None else C.c_void_p(v) for v in (gamma, beta))
+        for ws in (1 << 20, (1 << 20) - (need - 1) // 256 * 256):
+            rc = l.glowb200_group_norm(far, 1, None, 1.0, 0, far2, 1, g, b, 2, pixels, 64, 8, 1e-5, 0, C.c_void_p(ws), 1 << 20, None, None)
+            assert over(l, rc), (gamma, beta, ws)
