@@ -4,7 +4,8 @@
 //
 // mean and var over the C / G channels of the group and all pixels of the image.  Variances come from squares of
 // differences from a mean, never from a difference of two large sums: a thread takes a few pixels at a time, with their
-// own mean, and what two parts of a group know of themselves (n, mean, M2 = the sum of squared differences) is joined by
+// own mean (norm_any_*: a block its share of a group, in two passes), and what two parts of a group know of themselves
+// (n, mean, M2 = the sum of squared differences) is joined by
 //   M2 = M2a + M2b + (mean_b - mean_a)^2 na nb / (na + nb),
 // in an order that depends on the sizes alone.
 //
@@ -670,15 +671,26 @@ __global__ void __launch_bounds__(256) norm_any_parts_kernel(const NormParams p)
   const int g = (int)(ng - n * p.groups), width = p.channels / p.groups;
   const int64_t first = chunk * p.chunk_pixels, last = min(first + p.chunk_pixels, p.pixels), count = (last - first) * width;
   const T *x = reinterpret_cast<const T *>(p.in) + (n * p.pixels + first) * p.channels + g * width;
-  float sum = 0.0f;
-  for (int64_t i = threadIdx.x; i < count; i += 256) sum += to_float(x[i / width * p.channels + i % width]);
-  const float mean = block_sum(sum, shared) / (float)count;
-  float squares = 0.0f;
-  for (int64_t i = threadIdx.x; i < count; i += 256) {
-    const float d = to_float(x[i / width * p.channels + i % width]) - mean;
-    squares += d * d;
-  }
-  squares = block_sum(squares, shared);
+  // What the numbers less `from` and their squares add up to, 64 elements of a thread at a time: a long group is not one long chain.
+  auto sums_from = [&](float from) {
+    float2 sums = make_float2(0.0f, 0.0f);
+    for (int64_t i = threadIdx.x; i < count;) {
+      float2 few = make_float2(0.0f, 0.0f);
+      for (int k = 0; k < 64 && i < count; k++, i += 256) {
+        const float d = to_float(x[i / width * p.channels + i % width]) - from;
+        few.x += d;
+        few.y += d * d;
+      }
+      sums.x += few.x;
+      sums.y += few.y;
+    }
+    return make_float2(block_sum(sums.x, shared), block_sum(sums.y, shared));
+  };
+  // `about` is off by its sum's roundings, the same way in every thread where numbers hardly differ; what the differences from it add
+  // up to takes that out of the mean, and out of the squares (which are never fewer than its share).
+  const float about = sums_from(0.0f).x / (float)count;
+  const float2 sums = sums_from(about);
+  const float rest = sums.x / (float)count, share = sums.x * rest, mean = about + rest, squares = sums.y <= share ? 0.0f : sums.y - share;
   if (threadIdx.x == 0) p.partial[blockIdx.x] = make_float2(mean, squares);
 }
 

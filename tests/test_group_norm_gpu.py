@@ -221,3 +221,14 @@ def test_slices_whose_pieces_do_not_divide_a_block(shape, G, dtype):
     y, off = wanted(x, G, gamma, beta, 1e-5, "none", torch.finfo(x.dtype).eps / 2)
     tiny = torch.finfo(x.dtype).smallest_normal * torch.finfo(x.dtype).eps
     assert ((got.double() - y).abs() <= off + tiny).all()
+
+
+@pytest.mark.parametrize("value", [1000.03, 3.3])
+@pytest.mark.parametrize("shape,G", [((1184, 128, 513), 1), ((37, 1000, 4096), 32), ((1, 3000, 513), 27)])
+def test_a_constant_far_from_zero_with_a_block_to_a_group(shape, G, value):
+    """Pixels of more pieces than a block has threads: one block adds up a whole group.  Whatever its sum of equal numbers is off by,
+    the sum of their exact differences from the quotient takes it out again, up to a few times (the sums' depth * 2^-24)^2, so the
+    mean is off by its own rounding alone, less than a unit in its last place (2^-23), and nothing is left of the variance."""
+    x = torch.full(shape, value, device=DEV)
+    got = ops.group_norm(x, G)
+    assert float(got.abs().max()) <= 2.0 ** -23 * value / 1e-5 ** 0.5
