@@ -662,7 +662,8 @@ def microscaled_fp4_fc(inp, inp_scales, weights, weights_scales, bias=None, *, f
 def dynamic_microscaled_fp4_fc(inp, weights, weights_scales, bias=None, *, flags=0, out_dtype=None, out=None, workspace=None,
                                status=None):
     """microscaled_fp4_fc on a float input [M, K] (float32, float16 or bfloat16, rows may be apart) that the layer quantizes
-    itself; result [M, N] of out_dtype, by default the input's."""
+    itself, to the same operand as microscaled_fp4_quantize; result [M, N] of out_dtype, by default the input's.  The fp32 sums
+    may have another order than microscaled_fp4_fc's: results are equal where every partial sum is an fp32 number."""
     return _native().mx_dynamic_fc(inp, weights, weights_scales, bias, flags, _float_type(out_dtype), out, workspace, status)
 
 

@@ -677,9 +677,11 @@ int glowb200_microscaled_fp4_dequantize(const uint8_t *data, const uint8_t *scal
 int glowb200_microscaled_fp4_fc(void *out, int out_type, const uint8_t *in, const uint8_t *in_scales, const uint8_t *weights,
                                 const uint8_t *weights_scales, const float *bias, int64_t M, int64_t K, int64_t N, int flags,
                                 int32_t *status, glowb200_stream_t stream);
-/* The same with a float input [M,K] of in_type (rows `row_stride` elements apart), quantized by the layer: the result of
- * glowb200_microscaled_fp4_quantize followed by glowb200_microscaled_fp4_fc, bit for bit.  The workspace (256-byte
- * aligned) must hold glowb200_dynamic_microscaled_fp4_fc_workspace_bytes(M, K, N). */
+/* The same with a float input [M,K] of in_type (rows `row_stride` elements apart), quantized by the layer: the product's operand
+ * is what glowb200_microscaled_fp4_quantize writes, bit for bit.  The order of the fp32 sums follows from M, K and N, but for
+ * some of them not as in glowb200_microscaled_fp4_fc: results of the two are equal where fp32 holds every partial sum, and
+ * differ by the roundings of those additions elsewhere.  So do a row's results in products of different M.  The workspace
+ * (256-byte aligned) must hold glowb200_dynamic_microscaled_fp4_fc_workspace_bytes(M, K, N). */
 size_t glowb200_dynamic_microscaled_fp4_fc_workspace_bytes(int64_t M, int64_t K, int64_t N);
 int glowb200_dynamic_microscaled_fp4_fc(void *out, int out_type, const void *in, int in_type, int64_t row_stride,
                                         const uint8_t *weights, const uint8_t *weights_scales, const float *bias, int64_t M,

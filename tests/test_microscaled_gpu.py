@@ -345,3 +345,22 @@ def test_refusals():
     off = torch.empty(8 * 32 + 8, dtype=torch.uint8, device=DEV)[8:].view(8, 32)
     with pytest.raises(_lib.GlowB200Error, match="16-byte"):
         ops.microscaled_fp4_fc(off, s, w, ws)
+
+
+@pytest.mark.parametrize("M,K,N", [(16, 4096, 4096), (20, 2048, 512), (16, 1024, 8320), (8, 4096, 16384), (24, 4096, 6000), (32, 1024, 1024)])
+def test_dynamic_fc_where_the_two_layers_add_in_another_order(M, K, N):
+    """The depth in another number of parts, or another kernel than for the packed input: equal where fp32 holds all sums, and
+    within the roundings of K additions and of one number more a part (at most one unit in the last place each) elsewhere."""
+    a, sa, _ = operand(M + K, M, K, 1)
+    b, sb, _ = operand(N + K, N, K, 1)
+    x, w = ops.microscaled_fp4_dequantize(a, sa, K), ops.microscaled_fp4_dequantize(b, sb, K).double()
+    assert K * 12 * 12 * 16 < 2 ** 24  # products are multiples of 1 / 16, of numbers up to 12
+    got = ops.dynamic_microscaled_fp4_fc(x, b, sb, out_dtype=torch.float32)
+    assert torch.equal(got, ops.microscaled_fp4_fc(a, sa, b, sb, out_dtype=torch.float32)) and torch.equal(got.double(), x.double() @ w.T)
+    g = torch.Generator(device=DEV).manual_seed(M)
+    x = torch.randn(M, K, device=DEV, generator=g) * torch.exp(4 * torch.randn(M, K, device=DEV, generator=g))
+    a, sa = ops.microscaled_fp4_quantize(x)
+    x = ops.microscaled_fp4_dequantize(a, sa, K).double()
+    want, size = x @ w.T, x.abs() @ w.abs().T
+    for got in (ops.dynamic_microscaled_fp4_fc(x.float(), b, sb, out_dtype=torch.float32), ops.microscaled_fp4_fc(a, sa, b, sb, out_dtype=torch.float32)):
+        assert ((got.double() - want).abs() <= (K + 8) * 2.0 ** -23 * size).all()
