@@ -200,6 +200,7 @@ fp4_few_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
     const long long t0 = clock64();
     while (clock64() - t0 < 4000000ll) {
     }
+    __syncthreads();  // (each thread's loop ends for itself; what follows takes whole warps)
   }
   if (p.splits > 1) cluster_sync();
   tc_fence_after();
