@@ -61,10 +61,6 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi, __nv_bfloat16) {
   return r;
 }
 
-// Byte of the scale of row r, block b in a matrix of `tiles` scale tiles to a row.
-__device__ __forceinline__ int64_t mx_scale_at(int64_t r, int64_t b, int64_t tiles) {
-  return ((r >> 7) * tiles + (b >> 2)) * 512 + (r & 31) * 16 + ((r >> 5) & 3) * 4 + (b & 3);
-}
 // Scale byte of a block whose largest magnitude has these fp32 bits (sign bit clear): the biased exponent less two is
 // e + 127; infinities and NaNs have exponent 255.  (Magnitudes below 2^-124, subnormal ones too, take the smallest scale.)
 __device__ __forceinline__ uint32_t mx_scale_byte(uint32_t top) {
