@@ -7,7 +7,7 @@
 // own mean (norm_any_*: a block its share of a group, in two passes), and what two parts of a group know of themselves
 // (n, mean, M2 = the sum of squared differences) is joined by
 //   M2 = M2a + M2b + (mean_b - mean_a)^2 na nb / (na + nb),
-// in an order that depends on the sizes alone.
+// in an order that depends on the sizes and on the tensors' alignment alone.
 //
 // Three ways, by size:
 //   - one launch (norm_single_kernel) where a slice of 64 bytes of every pixel, whole groups, of one image lies in the shared
@@ -17,9 +17,14 @@
 //     launches 60).  128 bytes of a pixel take 52 there, 32 bytes 56, twice the blocks 57.
 //   - two launches (norm_stats_kernel, norm_chunks_kernel) for larger images: statistics of chunks of whole pixels, then a
 //     pass that joins them and normalises, from the last chunk and the last pixels to the first: what the first pass read
-//     last is still in L2 (126 MB).  Bound by bytes: 8 x 256 x 256 x 128 fp16 70 us, of which the statistics take 24 (134 MB at
-//     5.6 TB/s) and the rest moves 268 MB through L2 at the rate of a copy; Swish adds 5.
-//   - any number of channels a pixel (norm_any_*): three plain launches.
+//     last is still in L2 (126 MB).  8 x 256 x 256 x 128 fp16 70 us, 24 of them the statistics; Swish adds 5.  Bound by latency
+//     rather than by bytes or issue slots: on 4 images the passes move 3.7 and 3.1 TB/s of DRAM with 40 % of the issue slots used.  An SM has two
+//     blocks of 256 threads (registers, and the ring's shared memory), which wait for their stages (3.3 and 4.0 of 9.8 cycles to
+//     an instruction), and none at all for a quarter of the time, at either end of a launch.
+//   - any number of channels a pixel (norm_any_*): three plain launches, an element to a thread at a time, whose 64-bit quotients
+//     for places bound them: 8 x 32 x 32 x 8192 fp16 679 us, of which the bytes would take 42.
+// An int8 result costs a division and a conversion by 64 bits to an element, as the Quantize node rounds: 64 x 56 x 56 x 256 fp16
+// 169 us (float 48), 8 x 256 x 256 x 128 bf16 with Swish 204 (75); quotients of the zeros that Relu leaves are the slowest (247).
 #include "group_norm_plan.h"
 #include "microscaled.cuh"
 #include "tcgen05.cuh"
@@ -167,7 +172,8 @@ __device__ __forceinline__ void activate(float (&y)[N], int act) {
     for (int k = 0; k < N; k++) asm("max.NaN.f32 %0, %0, %1;" : "+f"(y[k]) : "f"(0.0f));
   } else if (act == GLOWB200_NORM_ACT_SWISH) {
     if constexpr (sizeof(Out) == 2) {
-      // (16-bit results: the approximate exponential and reciprocal are off by some 2^-21)
+      // (16-bit results: exponential and reciprocal are approximate, off by some 2^-21 of the result, and the product in front of
+      // them is rounded, which is |y| 2^-24 of it: 2^-18 at y = -80.  Both are lost in the rounding to come, 2^-9 or 2^-12.)
 #pragma unroll
       for (int k = 0; k < N; k++) {
         float e;
